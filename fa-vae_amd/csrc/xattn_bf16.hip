@@ -1,0 +1,4 @@
+// Cross attention, bf16 elements: the kernels of xattn.h for this type.
+#include "xattn_launch.h"
+
+XATTN_INSTANTIATE(BF16)

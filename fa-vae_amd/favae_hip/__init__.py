@@ -33,7 +33,7 @@ HW_QUEUES_AT_INIT = None if torch.cuda.is_initialized() else _parse_queues(os.en
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FAVAE_HIP_LIB") or os.path.join(_HERE, "libfavae_hip.so")     # FAVAE_HIP_LIB: same-box A/B of two builds
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 GATHER_PLAIN, GATHER_UPSAMPLE2, GATHER_DILATE2 = 0, 1, 2
 ACT_NONE, ACT_SILU, ACT_LEAKY02, ACT_RELU = 0, 1, 2, 3
@@ -54,6 +54,11 @@ class WinoJob(Structure):          # include/favae_hip.h favae_wino_job
 
 class ReduceJob(Structure):
     _fields_ = [("part", c_void_p), ("out", c_void_p), ("n", c_int64), ("slabs", c_int32), ("accumulate", c_int32)]
+
+
+class XattnDesc(Structure):        # include/favae_hip.h favae_xattn_desc
+    _fields_ = ([(n, c_int32) for n in ("B", "Lq", "Lk", "H", "Hkv", "D", "dtype")] + [("scale", c_float)] +
+                [(n, c_int64) for n in ("q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl", "v_sh", "pad_sb")])
 
 
 # name -> (restype, argtypes); mirrors include/favae_hip.h one to one (tests/test_abi.py checks the symbol list)
@@ -160,6 +165,13 @@ SIGNATURES = {
     "favae_wino_weights_bytes": (c_size_t, [c_int, c_int]),
     "favae_wino_weights": (c_int, [_P, _P, c_int, c_int, c_int, _P, _S]),
     "favae_segment_absmax": (c_int, [_P, _P, c_int, _P, _P, c_int, _P, _S]),
+    "favae_xattn_fwd_workspace": (c_size_t, [POINTER(XattnDesc)]),
+    "favae_xattn_fwd": (c_int, [POINTER(XattnDesc), _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _S]),
+    "favae_xattn_bwd_workspace": (c_size_t, [POINTER(XattnDesc)]),
+    "favae_xattn_bwd": (c_int, [POINTER(XattnDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, _S]),
+    "favae_embed_fwd": (c_int, [_P, c_int, _P, c_int64, c_int64, _P, c_int64, c_int, c_int, c_float, _S]),
+    "favae_embed_bwd_workspace": (c_size_t, [c_int64, c_int64, c_int]),
+    "favae_embed_bwd": (c_int, [_P, c_int, _P, c_int64, c_int64, c_int, c_int, c_float, c_int64, _P, _P, c_size_t, _S]),
     "favae_prof_enable": (c_int, [c_int]),
     "favae_prof_reset": (c_int, []),
     "favae_prof_report": (c_int64, [ctypes.c_char_p, c_int64]),

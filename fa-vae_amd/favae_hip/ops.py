@@ -5,14 +5,16 @@ code reads like the reference's NCHW code while every kernel sees coalesced chan
 """
 from __future__ import annotations
 
+import functools
 import math
 import ctypes
 import os
 from ctypes import byref
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from . import (ACT_LEAKY02, ACT_NONE, ACT_RELU, ACT_SILU, GATHER_DILATE2, GATHER_PLAIN, GATHER_UPSAMPLE2, ReduceJob, call,
+from . import (ACT_LEAKY02, ACT_NONE, ACT_RELU, ACT_SILU, GATHER_DILATE2, GATHER_PLAIN, GATHER_UPSAMPLE2, ReduceJob, XattnDesc, call,
                make_conv_desc, ptr, query, workspace)
 
 CL = torch.channels_last
@@ -1853,6 +1855,222 @@ class MHACoreFn(torch.autograd.Function):
 def mha_core(qkv, heads, p, training):
     p = float(p) if training else 0.0
     return MHACoreFn.apply(qkv, heads, p, _next_dropout_seed() if p > 0.0 else 0)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# conditioning on another sequence: token embedding and cross attention (fp32, bf16, fp16)
+# ---------------------------------------------------------------------------------------------------------------
+_DTYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # include/favae_hip.h FAVAE_DTYPE_*
+
+
+def _require_float_gpu(what, *tensors):
+    """all on one GPU and of one supported element type"""
+    t0 = tensors[0]
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError("favae_hip ops run on MI355X only (%s got a tensor on %s); there is no CPU fallback" % (what, t.device))
+        if t.dtype not in _DTYPE_ID:
+            raise RuntimeError("%s takes fp32, bf16 or fp16 tensors (got %s)" % (what, t.dtype))
+        if t.device != t0.device or t.dtype != t0.dtype:
+            raise RuntimeError("%s: tensors differ in device or type (%s %s, %s %s)" % (what, t0.device, t0.dtype, t.device, t.dtype))
+
+
+def _on_device(fn, device, *args):
+    """fn(*args) with `device` current: the stream a call goes to is the current one of the tensors' device"""
+    if device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+def _dense16(t):
+    """contiguous and 16-byte aligned (a copy where it is not)"""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _rows16(t):
+    """(B, L, H, D) with contiguous columns and 16-byte aligned rows (a dense copy where it has not)"""
+    unit = 16 // t.element_size()
+    sb, sl, sh, sd = t.stride()
+    return t if sd == 1 and not (sb % unit or sl % unit or sh % unit or t.data_ptr() % 16) else t.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=1024)
+def _xattn_desc(*fields):
+    """descriptor of these sizes and strides, with the workspace sizes of its two calls"""
+    d = XattnDesc(*fields)
+    return d, query("favae_xattn_fwd_workspace", byref(d)), query("favae_xattn_bwd_workspace", byref(d))
+
+
+def _xattn_plan(q, k, v, pad, scale):
+    B, Lq, H, D = q.shape
+    return _xattn_desc(B, Lq, k.shape[1], H, k.shape[2], D, _DTYPE_ID[q.dtype], scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                       0 if pad is None else pad.stride(0))
+
+
+def _xattn_fwd(q, k, v, pad, scale, with_grad):
+    """-> out, out before its rounding, row log-sums (the last two only for a backward pass)"""
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if q.numel() == 0 or k.shape[1] == 0:
+        return out.zero_(), None, None
+    d, nbytes, _ = _xattn_plan(q, k, v, pad, scale)
+    o32 = lse = ws = None
+    if with_grad:
+        o32 = out if out.dtype == torch.float32 else torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        lse = torch.empty((q.shape[0] * q.shape[1] * q.shape[2],), dtype=torch.float32, device=q.device)
+    if nbytes:
+        ws = workspace(nbytes, q.device)
+    call("favae_xattn_fwd", byref(d), ptr(q), ptr(k), ptr(v), ptr(pad), ptr(out), ptr(o32), ptr(lse), ptr(ws), nbytes)
+    return out, o32, lse
+
+
+def _xattn_bwd(q, k, v, pad, scale, o32, lse, dout, need_kv):
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if need_kv else None
+    dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if need_kv else None
+    d, _, nbytes = _xattn_plan(q, k, v, pad, scale)
+    ws = workspace(nbytes, q.device)
+    call("favae_xattn_bwd", byref(d), ptr(q), ptr(k), ptr(v), ptr(pad), ptr(o32), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(ws), nbytes)
+    return dq, dk, dv
+
+
+class CrossAttentionFn(torch.autograd.Function):
+    """Attention of one sequence's rows to another one's (cross_attention) with its backward pass.  Saved: the inputs, the output before
+    its rounding (delta = <dout, out> of a rounded output would carry the rounding into every score gradient) and the row log-sums; the
+    probabilities are formed again.  Shared key / value heads: their gradients are summed over the group inside the kernel."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, pad, scale):
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        out, o32, lse = _on_device(_xattn_fwd, q.device, q, k, v, pad, scale, True)
+        ctx.scale, ctx.same = scale, o32 is out
+        ctx.save_for_backward(q, k, v, pad, out if ctx.same else o32, lse)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, pad, o32, lse = ctx.saved_tensors
+        if lse is None:                                   # no row or no key: nothing depends on anything
+            return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)) + (None, None)
+        need_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dq, dk, dv = _on_device(_xattn_bwd, q.device, q, k, v, pad, ctx.scale, o32, lse, _dense16(dout), need_kv)
+        return dq, dk, dv, None, None
+
+
+def cross_attention(q, k, v, key_padding_mask=None, scale=None):
+    """softmax(scale q k^T) v per head, where the keys and values come from another sequence than the queries (an encoder's states, a
+    prompt), of another length.  q (B, Lq, H, D); k, v (B, Lk, Hkv, D) with H a multiple of Hkv: query head h reads key / value head
+    h // (H // Hkv).  fp32, bf16 or fp16, all alike; D a multiple of 8 up to 128; any strides (views of a packed projection and expanded
+    tensors are read in place where their rows are contiguous and 16-byte aligned, other layouts are copied first).
+    key_padding_mask: bool (B, Lk), True = this key is padding (nn.MultiheadAttention's meaning); a row that is left without keys gives
+    zeros, and whatever padded rows of k and v hold reaches no result.  scale: 1 / sqrt(D) unless given, positive.
+    Lq = 1 (a decoding step) and long keys run the same call: the keys are split over the chip.  Differentiable in q, k, v, once."""
+    _require_float_gpu("cross_attention", q, k, v)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError("cross_attention: q (B, Lq, H, D) and k, v (B, Lk, Hkv, D), got %s, %s, %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    B, Lq, H, D = q.shape
+    Hkv = k.shape[2]
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise ValueError("cross_attention: %d query heads do not share %d key / value heads evenly" % (H, Hkv))
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError("cross_attention: a head has a multiple of 8 columns, 8 to 128 (got %d)" % D)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("cross_attention: scale has to be positive and finite (got %r)" % scale)
+    if key_padding_mask is not None:
+        m = key_padding_mask
+        if m.dtype != torch.bool or tuple(m.shape) != (B, k.shape[1]) or m.device != q.device:
+            raise ValueError("cross_attention: key_padding_mask is a bool tensor (B, Lk) = %s on %s, got %s %s on %s"
+                             % ((B, k.shape[1]), q.device, m.dtype, tuple(m.shape), m.device))
+        if m.stride(1) != 1 and m.shape[1] > 1:
+            m = m.contiguous()
+        key_padding_mask = m
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return CrossAttentionFn.apply(q, k, v, key_padding_mask, scale)
+    return _on_device(_xattn_fwd, q.device, _rows16(q), _rows16(k), _rows16(v), key_padding_mask, scale, False)[0]
+
+
+def _check_ids(what, ids, device):
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError("%s: ids are int64 or int32 (got %s)" % (what, ids.dtype))
+    if ids.device != device:
+        raise RuntimeError("%s: ids on %s, rows on %s" % (what, ids.device, device))
+    return ids if ids.is_contiguous() else ids.contiguous()
+
+
+def _check_padding_idx(what, padding_idx, rows):
+    if padding_idx is None:
+        return -1
+    p = int(padding_idx) + (rows if padding_idx < 0 else 0)
+    if not 0 <= p < rows:
+        raise ValueError("%s: padding_idx %d of a table of %d rows" % (what, padding_idx, rows))
+    return p
+
+
+def _embed_fwd(ids, weight, scale):
+    V, C = weight.shape
+    out = torch.empty((*ids.shape, C), dtype=weight.dtype, device=weight.device)
+    if out.numel():
+        call("favae_embed_fwd", ptr(ids), ids.dtype == torch.int64, ptr(weight), weight.stride(0), V, ptr(out), ids.numel(), C,
+             _DTYPE_ID[weight.dtype], scale)
+    return out
+
+
+def _embed_bwd(dout, ids, rows, scale, padding):
+    C = dout.shape[-1]
+    dw = torch.empty((rows, C), dtype=dout.dtype, device=dout.device)
+    if dout.numel() == 0:
+        return dw.zero_()
+    ws = workspace(query("favae_embed_bwd_workspace", ids.numel(), rows, C), dout.device)
+    call("favae_embed_bwd", ptr(ids), ids.dtype == torch.int64, ptr(dout), ids.numel(), rows, C, _DTYPE_ID[dout.dtype], scale, padding,
+         ptr(dw), ptr(ws), ws.numel())
+    return dw
+
+
+class EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding):
+        ctx.rows, ctx.scale, ctx.padding = weight.shape[0], scale, padding
+        ctx.save_for_backward(ids)
+        return _on_device(_embed_fwd, weight.device, ids, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        return _on_device(_embed_bwd, dout.device, _dense16(dout), ids, ctx.rows, ctx.scale, ctx.padding), None, None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """scale * weight[ids]: ids (int64 or int32, any shape), weight (V, C) fp32, bf16 or fp16 -> (*ids.shape, C), one rounding.  The row
+    padding_idx is looked up like any other and gets no gradient (nn.Embedding).  An id outside [0, V) reads nothing and gives a row of
+    NaN: ids stay on the device, so nothing can be raised without waiting for it.  Differentiable in weight, once (embedding_grad)."""
+    _require_float_gpu("embedding", weight)
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError("embedding: weight is (V, C), got %s" % (tuple(weight.shape),))
+    ids = _check_ids("embedding", ids, weight.device)
+    padding = _check_padding_idx("embedding", padding_idx, weight.shape[0])
+    scale = float(scale)
+    if weight.stride(1) != 1 and weight.shape[1] > 1:
+        weight = weight.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return EmbeddingFn.apply(weight, ids, scale, padding)
+    return _on_device(_embed_fwd, weight.device, ids, weight, scale)
+
+
+def embedding_grad(dout, ids, rows, scale=1.0, padding_idx=None):
+    """Gradient of embedding() with respect to its table of `rows` rows: (rows, C) with scale * the sum of dout[t] over ids[t] == v in row
+    v (fp32 sums in a fixed order, rounded once), zeros where no token names the row or v == padding_idx.  Tokens are sorted by id
+    (stable); nothing is added atomically.  The call under embedding()'s backward pass, for programs that keep gradients themselves."""
+    _require_float_gpu("embedding_grad", dout)
+    rows = int(rows)
+    if rows < 1 or dout.dim() < 1 or dout.shape[:-1] != ids.shape or dout.shape[-1] < 1:
+        raise ValueError("embedding_grad: dout (*ids.shape, C) and at least one row, got %s for ids %s and %d rows"
+                         % (tuple(dout.shape), tuple(ids.shape), rows))
+    ids = _check_ids("embedding_grad", ids, dout.device)
+    padding = _check_padding_idx("embedding_grad", padding_idx, rows)
+    return _on_device(_embed_bwd, dout.device, _dense16(dout), ids, rows, float(scale), padding)
 
 
 # ---------------------------------------------------------------------------------------------------------------

@@ -125,6 +125,32 @@ class AttnBlock(nn.Module):
         return K.fused_conv(o, a.out_proj.weight, a.out_proj.bias, resid=xa, cfg=_C1)
 
 
+class CrossAttnBlock(nn.Module):
+    """Image tokens attend to the states of another sequence: x + proj(attention(q(GroupNorm(x)), kv(states))).  The reference has no such
+    block (its codec attends within the image); it is laid out like AttnBlock and TransEncoderBlock (GroupNorm(32), 8 heads): the
+    projections are 1x1 convs, the two halves of `kv` are read in place.  states (B, L, ctx_c) of any length; padding (B, L) bool, True =
+    not a token (nn.MultiheadAttention's key_padding_mask).  An image whose states are all padding passes through with proj's bias."""
+
+    def __init__(self, in_c, ctx_c, num_heads=8):
+        super().__init__()
+        if in_c % num_heads or in_c // num_heads % 8 or in_c // num_heads > 128:
+            raise ValueError("CrossAttnBlock: %d channels in %d heads: a head has a multiple of 8 channels, at most 128" % (in_c, num_heads))
+        self.num_heads = num_heads
+        self.norm = nn.GroupNorm(32, in_c)
+        self.q = nn.Linear(in_c, in_c)
+        self.kv = nn.Linear(ctx_c, 2 * in_c)
+        self.proj = nn.Linear(in_c, in_c)
+        self._cfg_in = K.ConvCfg(1, 1, 1, 0, act=ACT_NONE, groups=32)
+
+    def forward(self, x, states, padding=None):
+        q, xa = K.fused_conv(x, self.q.weight, self.q.bias, self.norm.weight, self.norm.bias, None, self._cfg_in, True)
+        B, C, H, W = q.shape
+        kv = K.fused_conv(states.transpose(1, 2).unsqueeze(2), self.kv.weight, self.kv.bias, cfg=_C1)      # (B, 2C, 1, L)
+        k, v = kv.permute(0, 2, 3, 1).reshape(B, -1, 2, self.num_heads, C // self.num_heads).unbind(2)
+        o = K.cross_attention(q.permute(0, 2, 3, 1).reshape(B, H * W, self.num_heads, -1), k, v, padding)
+        return K.fused_conv(o.view(B, H, W, C).permute(0, 3, 1, 2), self.proj.weight, self.proj.bias, resid=xa, cfg=_C1)
+
+
 class TransEncoderBlock(nn.Module):
     """FCM with attention architecture (codec.py:108-122): GroupNorm(32) -> nn.TransformerEncoderLayer(in_c, nhead=8,
     batch_first=True) on the (B, HW, C) tokens -> back to (B, C, H, W).  The layer's defaults are what the reference gets:

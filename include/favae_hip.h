@@ -506,6 +506,45 @@ int favae_gn_act_bwd_tiles(const float* da, const float* x, const float* gamma, 
                            favae_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * Conditioning on another sequence (no reference counterpart on this path: its transformer attends within one sequence,
+ * models/codec.py:92,112): the embedding of that sequence's tokens and the attention of image tokens to its states.
+ * Element types: 0 fp32, 1 bf16, 2 fp16.  All sums, softmax statistics and norms are fp32; a result is rounded once.
+ * ---------------------------------------------------------------------------------------------------------- */
+#define FAVAE_DTYPE_F32 0
+#define FAVAE_DTYPE_BF16 1
+#define FAVAE_DTYPE_F16 2
+/* Cross attention: q, o, dout, dq (B, Lq, H, D), k, v, dk, dv (B, Lk, Hkv, D); query head h reads key / value head h / (H / Hkv).
+ *   o = softmax over the keys of scale * <q, k> that are not padding, times v; a row without keys gives zeros, and zero gradients.
+ * Strides are in elements, for q, k, v (batch, length, head; columns contiguous, each stride a multiple of 16 bytes, 0 allowed); o, dout
+ * and the gradients are dense.  D % 8 == 0, 8 <= D <= 128, scale > 0.  key_padding_mask: NULL, or B rows of Lk bytes pad_sb bytes apart,
+ * nonzero = this key is padding: what its rows of k and v hold (infinities, NaN) reaches no result and its gradients are zeros.
+ * Every data pointer is 16-byte aligned.  Results do not depend on anything but the arguments (no atomics on floats). */
+typedef struct {
+    int32_t B, Lq, Lk, H, Hkv, D, dtype;
+    float scale;
+    int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, pad_sb;
+} favae_xattn_desc;
+/* Forward.  o32 (may be NULL): o before its rounding, fp32; lse (may be NULL): B * H * Lq floats.  The backward pass wants both (for
+ * fp32 elements o32 may be o itself).  Workspace: 0 bytes unless few rows attend to many keys (the keys are then split). */
+size_t favae_xattn_fwd_workspace(const favae_xattn_desc* d);
+int favae_xattn_fwd(const favae_xattn_desc* d, const void* q, const void* k, const void* v, const uint8_t* key_padding_mask, void* o,
+                    float* o32, float* lse, void* ws, size_t ws_bytes, favae_stream_t stream);
+/* Backward from o32 and lse of the forward call with the same descriptor.  dk and dv may be NULL together. */
+size_t favae_xattn_bwd_workspace(const favae_xattn_desc* d);
+int favae_xattn_bwd(const favae_xattn_desc* d, const void* q, const void* k, const void* v, const uint8_t* key_padding_mask,
+                    const float* o32, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes,
+                    favae_stream_t stream);
+/* Token embedding: out[t][c] = scale * weight[ids[t]][c] for T ids (int32, or int64 where ids_are_64bit != 0) and V rows weight_stride
+ * elements apart; out is dense.  An id outside [0, V) reads nothing and gives a row of NaN. */
+int favae_embed_fwd(const void* ids, int ids_are_64bit, const void* weight, int64_t weight_stride, int64_t V, void* out, int64_t T, int C,
+                    int dtype, float scale, favae_stream_t stream);
+/* Its gradient: dweight[v][c] = scale * sum of dout[t][c] over the t with ids[t] == v, all V rows written (dense, 16-byte aligned).  Ids
+ * outside [0, V) and ids equal to padding_idx (-1: none) contribute nothing.  Equal ids are summed in a fixed order. */
+size_t favae_embed_bwd_workspace(int64_t T, int64_t V, int C);
+int favae_embed_bwd(const void* ids, int ids_are_64bit, const void* dout, int64_t T, int64_t V, int C, int dtype, float scale,
+                    int64_t padding_idx, void* dweight, void* ws, size_t ws_bytes, favae_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------------------
  * Launch profiler (measurement only; no reference counterpart -- the reference is timed from outside by its caller).
  * level 0: off (default).  level 1: every launch that carries >= 1 GFLOP of algorithmic work (the matrix-bound conv forward /
  * data-gradient / weight-gradient kernels) is bracketed by two HIP events recorded on ITS launch stream; level 2: every launch of
