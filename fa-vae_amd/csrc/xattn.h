@@ -4,7 +4,7 @@
 //
 // One pass over the keys with a running maximum and sum (no score matrix in memory).  Every product is a 32x32x16 16-bit MFMA:
 //   * the streamed operand (K, V forward and dQ; Q, dO for dK / dV) is staged row-major in LDS; as an MFMA A operand its rows are read
-//     with ds_read_b128, transposed with ds_read_b64_tr_b16 (4 rows x 16 columns per 16 lanes);
+//     with ds_read_b128, transposed with ds_read_b64_tr_b16 (4 rows x 16 columns per 16 lanes), both without bank conflicts (swizzle());
 //   * the stationary operand sits in registers as B operand, so that a score tile comes out TRANSPOSED: lane l owns query (or key)
 //     l % 32 and holds 16 scores of it.  Row statistics are per-lane scalars (one lane exchange per tile), and the tile's registers are,
 //     packed, the B operand of the next product: contraction slot (l / 32, j) of step s is row 16 s + 8 (j / 4) + 4 (l / 32) + j % 4 of
@@ -48,8 +48,10 @@ template <int TY> struct Ty {
     static constexpr int PL = TY == F32 ? 3 : 1;         // planes of an operand
     static constexpr int ES = TY == F32 ? 4 : 2;         // bytes of an element
     static constexpr int EPC = 16 / ES;                  // elements of a 16-byte chunk
-    // fp16 keeps 5 exponent bits: probabilities (<= 1) are formed times 2^15, so that one of 2^-29 is still a normal number
+    // fp16 keeps 5 exponent bits.  Backward, probabilities (<= 1) are formed times 2^15, so that one of 2^-29 is still a normal number;
+    // forward they may exceed 1 by 2^LAZY (fwd_kernel) and are formed times 2^7.
     static constexpr float PSHIFT = TY == F16 ? 15.f : 0.f;
+    static constexpr float FSHIFT = TY == F16 ? 7.f : 0.f;
 };
 
 template <int PL> struct Frag { s16x8 p[PL]; };
@@ -128,18 +130,26 @@ __device__ __forceinline__ f32x16 zero16() {
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// ---- LDS tiles: PL planes of ROWS rows of DP + 8 16-bit values.  The 16 bytes behind each row put the rows that one phase of a 128-bit
-// read touches on different banks (row stride 4 * odd dwords). -----------------------------------------------------------------------
-template <int DP> constexpr int row_len() { return DP + 8; }
-template <int TY, int DP, int ROWS> constexpr int tile_len() { return Ty<TY>::PL * ROWS * row_len<DP>(); }   // in 16-bit values
+// ---- LDS tiles: PL planes of ROWS rows of DP 16-bit values, the 16-byte chunks of a row permuted --------------------------------------
+// LDS has 64 banks of 4 bytes; a row covers DP / 2 of them.  A 128-bit read serves the same chunk of 16 rows at once (lanes {0-3, 12-15,
+// 20-27}, {4-11, 16-19, 28-31} and these + 32), a transposing 64-bit read four chunks of 4 rows (lanes 0-31, 32-63).  Chunk c of row r is
+// stored at c ^ swizzle(r), which spreads both over all banks for every DP (rows padded by 16 bytes instead: 2 to 4 lanes a bank on the
+// transposed reads).  swizzle(r + 16) == swizzle(r), so a lane's addresses differ by constants between groups of 16 rows.
+template <int DP> __device__ __forceinline__ int swizzle(int r) {
+    if constexpr (DP == 64) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+    else if constexpr (DP == 128) return (r & 3) << 2 | ((r >> 2) & 3);
+    else return (r >> 2) & 3;                            // 32, 96: row starts already differ by quarters of the banks
+}
+template <int TY, int DP, int ROWS> constexpr int tile_len() { return Ty<TY>::PL * ROWS * DP; }      // in 16-bit values
 
 // A operand, rows as they are: lane l holds row row0 + l % 32, columns col0 + 8 (l / 32) + 0..7
 template <int TY, int DP, int ROWS>
 __device__ __forceinline__ Frag<Ty<TY>::PL> row_frag(const short* t, int row0, int col0, int lane) {
     Frag<Ty<TY>::PL> f;
-    const short* p = t + (row0 + (lane & 31)) * row_len<DP>() + col0 + 8 * (lane >> 5);
+    const int r = lane & 31;
+    const short* p = t + r * DP + 8 * ((col0 / 8 + (lane >> 5)) ^ swizzle<DP>(r)) + row0 * DP;
 #pragma unroll
-    for (int i = 0; i < Ty<TY>::PL; ++i) f.p[i] = *reinterpret_cast<const s16x8*>(p + i * ROWS * row_len<DP>());
+    for (int i = 0; i < Ty<TY>::PL; ++i) f.p[i] = *reinterpret_cast<const s16x8*>(p + i * ROWS * DP);
     return f;
 }
 // A operand, transposed: lane l holds column col0 + l % 32, contraction slot j = row row0 + 8 (j / 4) + 4 (l / 32) + j % 4
@@ -147,84 +157,123 @@ template <int TY, int DP, int ROWS>
 __device__ __forceinline__ Frag<Ty<TY>::PL> col_frag(short* t, int row0, int col0, int lane) {
     typedef __attribute__((address_space(3))) s16x4* lds4;
     Frag<Ty<TY>::PL> f;
-    short* p = t + (row0 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * row_len<DP>() + col0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2), c = col0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    short* p = t + r * DP + 8 * (c ^ swizzle<DP>(r)) + 4 * (lane & 1) + row0 * DP;
+    short* q = t + (r + 8) * DP + 8 * (c ^ swizzle<DP>(r + 8)) + 4 * (lane & 1) + row0 * DP;
 #pragma unroll
     for (int i = 0; i < Ty<TY>::PL; ++i) {
-        short* pi = p + i * ROWS * row_len<DP>();
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)pi);
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(pi + 8 * row_len<DP>()));
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + i * ROWS * DP));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(q + i * ROWS * DP));
         f.p[i] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     return f;
 }
 
 // ---- staging: ROWS x DP elements through registers, NT threads, 16-byte chunks ---------------------------------------------------------
+// Rows `stride` bytes apart from a wave-uniform base; a lane's offsets are 32 bits (the entry point refuses strides of 2^24 bytes and
+// more), rows behind the end and columns behind D read zeros by the buffer's bound.
 template <int TY, int DP, int ROWS, int NT> struct Stage {
     static constexpr int CPR = DP / Ty<TY>::EPC;         // chunks of a row
     static constexpr int N = (ROWS * CPR + NT - 1) / NT; // chunks of a thread
+    static constexpr bool PART = ROWS * CPR % NT != 0;   // the last one not of every thread
     ux4 r[N];
-    // row_ptr(row) -> pointer to the row's elements or NULL (zeros instead)
-    template <typename F>
-    __device__ __forceinline__ void load(int tid, int D, F row_ptr) {
+    __device__ __forceinline__ static int row_of(int tid, int i) { return (tid + i * NT) / CPR; }
+    __device__ __forceinline__ static int col_of(int tid, int i) { return (tid + i * NT) % CPR * Ty<TY>::EPC; }
+    // rows [0, rows) of the tile exist; rows >= 1
+    __device__ __forceinline__ void load(int tid, int D, const char* base, int64_t stride, int rows) {
+        const int64_t bytes = rows * stride;
+        const auto rs = make_rsrc(base, (unsigned)(bytes < 0x7fffffff ? bytes : 0x7fffffff));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = tid + i * NT, row = id / CPR, col = (id % CPR) * Ty<TY>::EPC;
+            const unsigned off = (unsigned)row_of(tid, i) * (unsigned)stride + col_of(tid, i) * Ty<TY>::ES;
+            r[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, col_of(tid, i) >= D || (PART && row_of(tid, i) >= ROWS) ? FAVAE_OOB : off, 0, 0);
+        }
+    }
+    // any rows: row_ptr(row) -> pointer to the row's elements or NULL (zeros instead)
+    template <typename F>
+    __device__ __forceinline__ void gather(int tid, int D, F row_ptr) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
             ux4 x = {0u, 0u, 0u, 0u};
-            if (row < ROWS && col < D) {
-                const char* p = row_ptr(row);
-                if (p) x = *reinterpret_cast<const ux4*>(p + (size_t)col * Ty<TY>::ES);
+            if (col_of(tid, i) < D && (!PART || row_of(tid, i) < ROWS)) {
+                const char* p = row_ptr(row_of(tid, i));
+                if (p) x = *reinterpret_cast<const ux4*>(p + col_of(tid, i) * Ty<TY>::ES);
             }
             r[i] = x;
         }
     }
     // keep(row): false writes zeros, so that what stands in a padded row (an infinity, a NaN) reaches no product
     template <typename F>
-    __device__ __forceinline__ void store(short* t, int tid, F keep) const {
+    __device__ __forceinline__ void blank(int tid, F keep) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int id = tid + i * NT, row = id / CPR, col = (id % CPR) * Ty<TY>::EPC;
-            if (ROWS * CPR % NT && row >= ROWS) continue;
-            const bool kp = keep(row);
-            ux4 x = r[i];
+            const bool kp = (PART && row_of(tid, i) >= ROWS) || keep(row_of(tid, i));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = kp ? x[j] : 0u;
-            short* p = t + row * row_len<DP>() + col;
+            for (int j = 0; j < 4; ++j) r[i][j] = kp ? r[i][j] : 0u;
+        }
+    }
+    __device__ __forceinline__ void store(short* t, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = row_of(tid, i), col = col_of(tid, i);
+            if (PART && row >= ROWS) continue;
+            short* p = t + row * DP + 8 * ((col / 8) ^ swizzle<DP>(row)) + (col & 7);
             if constexpr (TY == F32) {
                 unsigned h0, m0, l0, h1, m1, l1;
-                const fx4 f = __builtin_bit_cast(fx4, x);
+                const fx4 f = __builtin_bit_cast(fx4, r[i]);
                 split2(f.x, f.y, h0, m0, l0);
                 split2(f.z, f.w, h1, m1, l1);
-                constexpr int PS = ROWS * row_len<DP>();
+                constexpr int PS = ROWS * DP;
                 *reinterpret_cast<uint2*>(p) = make_uint2(h0, h1);
                 *reinterpret_cast<uint2*>(p + PS) = make_uint2(m0, m1);
                 *reinterpret_cast<uint2*>(p + 2 * PS) = make_uint2(l0, l1);
             } else {
-                *reinterpret_cast<ux4*>(p) = x;
+                *reinterpret_cast<ux4*>(p) = r[i];
             }
         }
     }
 };
 
 // B operand of one row straight from memory: columns 16 s + 8 (l / 32) + 0..7 of every step s; p == NULL or columns behind D: zeros
-template <int TY, int DP>
-__device__ __forceinline__ void load_row(const void* p, int D, int lane, float (&f)[DP / 16][8]) {
+template <int DP>
+__device__ __forceinline__ void load_floats(const float* p, int D, int lane, float (&f)[DP / 16][8]) {
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
         const int col = 16 * s + 8 * (lane >> 5);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[s][j] = 0.f;
+        fx4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
         if (p && col < D) {
-            if constexpr (TY == F32) {
-                const fx4 a = reinterpret_cast<const fx4*>(p)[col / 4], b = reinterpret_cast<const fx4*>(p)[col / 4 + 1];
+            a = reinterpret_cast<const fx4*>(p)[col / 4];
+            b = reinterpret_cast<const fx4*>(p)[col / 4 + 1];
+        }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { f[s][j] = a[j]; f[s][4 + j] = b[j]; }
-            } else {
-                const ux4 u = reinterpret_cast<const ux4*>(p)[col / 8];
+        for (int j = 0; j < 4; ++j) { f[s][j] = a[j]; f[s][4 + j] = b[j]; }
+    }
+}
+template <int TY, int DP>
+__device__ __forceinline__ void load_row(const void* p, int D, int lane, Frag<Ty<TY>::PL> (&r)[DP / 16]) {
+    if constexpr (TY == F32) {
+        float f[DP / 16][8];
+        load_floats<DP>((const float*)p, D, lane, f);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { const fx2 w = unpack2<TY>(u[j]); f[s][2 * j] = w.x; f[s][2 * j + 1] = w.y; }
-            }
+        for (int s = 0; s < DP / 16; ++s) r[s] = make_frag<TY>(f[s]);
+    } else {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int col = 16 * s + 8 * (lane >> 5);
+            r[s].p[0] = (s16x8){0, 0, 0, 0, 0, 0, 0, 0};
+            if (p && col < D) r[s].p[0] = reinterpret_cast<const s16x8*>(p)[col / 8];
         }
     }
+}
+// element j of a fragment as a float (the three planes add up to it exactly)
+template <int TY> __device__ __forceinline__ float frag_at(const Frag<Ty<TY>::PL>& f, int j) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = Ty<TY>::PL - 1; i >= 0; --i) {
+        const short e = f.p[i][j];
+        x += unpack2<TY>((unsigned)(unsigned short)e).x;
+    }
+    return x;
 }
 
 // four consecutive elements
@@ -260,30 +309,60 @@ __device__ __forceinline__ int last_key(const uint8_t* pad, int k0, int k1, int 
     return last;
 }
 
+// two LDS buffers (one barrier a tile) where as many workgroups still fit a CU as its registers allow
+constexpr int bufs_of(int tile, int waves) { return 4 * tile * 2 <= (waves == 1 ? 150000 : 77000) ? 2 : 1; }
+// keys of a tile that take part: bit j of word i is key 64 i + j
+template <int BK> constexpr unsigned long long all_keys() { return BK >= 64 ? ~0ull : (1ull << (BK & 63)) - 1; }
+
+// key masks: a tile's scores start at 0 for a key and at -infinity for padding, as the accumulator of their first product
+__device__ __forceinline__ f32x16 start16(const float* bias, int half) {
+    f32x16 s;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const fx4 x = *reinterpret_cast<const fx4*>(bias + 8 * g + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * g + i] = x[i];
+    }
+    return s;
+}
+template <int TY, int DP, int ROWS>
+__device__ __forceinline__ f32x16 scores(const short* t, int row0, const Frag<Ty<TY>::PL> (&b)[DP / 16], bool all, const float* bias, int lane) {
+    const Frag<Ty<TY>::PL> f = row_frag<TY, DP, ROWS>(t, row0, 0, lane);
+    f32x16 s;
+    if (all) s = mma<TY>(f, b[0], zero16());
+    else s = mma<TY>(f, b[0], start16(bias, lane >> 5));
+#pragma unroll
+    for (int d = 1; d < DP / 16; ++d) s = mma<TY>(row_frag<TY, DP, ROWS>(t, row0, 16 * d, lane), b[d], s);
+    return s;
+}
+
 // -------------------------------------------------------------------------------------------------------------------------------------
-// Forward.  KEYW = false: 4 waves of 32 QS rows each share 64 keys a tile.  KEYW = true, for few rows: one 32-row tile per workgroup,
+// Forward.  KEYW = false: 4 waves of 32 rows each share 64 keys a tile.  KEYW = true, for few rows: one 32-row tile per workgroup,
 // each wave takes 32 other keys of the tile and the waves' results are joined at the end.
 // -------------------------------------------------------------------------------------------------------------------------------------
-template <int TY, int DP, int QS, bool KEYW> struct FwdCfg {
-    static constexpr int NW = KEYW && TY == F32 && DP > 64 ? 2 : 4;        // fp32 of 96, 128 columns: the planes of 128 keys do not fit
-    static constexpr int NT = 64 * NW;
-    static constexpr int ROWS = KEYW ? 32 : 32 * QS * NW;
-    static constexpr int BK = KEYW ? 32 * NW : 64;
-    static constexpr int KS = KEYW ? 1 : 2;
+constexpr float LAZY = 8.f;      // the running maximum follows only when a row's scores exceed it by 2^8: p <= 2^8, few rescalings
+
+template <int TY, int DP, bool KEYW> struct FwdCfg {
+    static constexpr int NT = 256;
+    static constexpr int NW = KEYW && TY == F32 && DP > 64 ? 2 : 4;        // waves that compute: the planes of 128 keys of 96, 128 fp32 columns
+    static constexpr int ROWS = KEYW ? 32 : 32 * NW;                       // do not fit LDS, there two waves only load
+    static constexpr int WAVES = TY == F32 && DP > 64 ? 1 : 2;            // a SIMD; also keeps accumulators out of the second register file
+    static constexpr int BK = KEYW ? 32 * NW : TY == F32 ? 32 : 64;
+    static constexpr int KS = KEYW ? 1 : BK / 32;
     static constexpr int TILE = tile_len<TY, DP, BK>();
+    static constexpr int BUFS = bufs_of(TILE, WAVES);
     static constexpr int RED = KEYW ? NW * DP * 32 * 2 : 0;               // joined results (fp32, in 16-bit units), over the tiles
-    static constexpr int LEN = 2 * TILE > RED ? 2 * TILE : RED;
-    static constexpr size_t LDS = LEN * 2 + 64 * 4 * NW + 16;
+    static constexpr int LEN = 2 * TILE * BUFS > RED ? 2 * TILE * BUFS : RED;
+    static constexpr size_t LDS = LEN * 2 + BUFS * BK * 4 + 64 * 4 * NW + 16;
 };
 
-template <int TY, int DP, int QS, bool KEYW>
-__global__ __launch_bounds__((FwdCfg<TY, DP, QS, KEYW>::NT)) void fwd_kernel(const Args a) {
-    using C = FwdCfg<TY, DP, QS, KEYW>;
+template <int TY, int DP, bool KEYW>
+__global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::WAVES)) void fwd_kernel(const Args a) {
+    using C = FwdCfg<TY, DP, KEYW>;
     using T = Ty<TY>;
     extern __shared__ __attribute__((aligned(16))) short lds[];
-    short* const kt = lds;
-    short* const vt = lds + C::TILE;
-    float* const stat = reinterpret_cast<float*>(lds + C::LEN);            // [2][NW][32] maxima, sums (KEYW)
+    float* const bias = reinterpret_cast<float*>(lds + C::LEN);           // [BUFS][BK]
+    float* const stat = bias + C::BUFS * C::BK;                           // [2][NW][32] maxima, sums (KEYW)
     int* const red = reinterpret_cast<int*>(stat + 64 * C::NW);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     int id = xcd_remap(blockIdx.x, gridDim.x);
@@ -295,116 +374,96 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, QS, KEYW>::NT)) void fwd_kernel(con
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
     const int k0 = split * a.span, kend = last_key<C::NT>(pad, k0, min(a.Lk, k0 + a.span), tid, red);
 
-    int row[QS];
-    Frag<T::PL> qf[QS][DP / 16];
-#pragma unroll
-    for (int u = 0; u < QS; ++u) {
-        row[u] = tile * C::ROWS + (KEYW ? 0 : 32 * QS * w) + 32 * u + (lane & 31);
-        float f[DP / 16][8];
-        load_row<TY, DP>(row[u] < a.R ? (const char*)a.q + row_at(a, bh, row[u], a.q_b, a.q_l, a.q_h) * T::ES : nullptr, a.D, lane, f);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) qf[u][s] = make_frag<TY>(f[s]);
-    }
-    f32x16 o[QS][DP / 32];
-    float m[QS], l[QS];
-#pragma unroll
-    for (int u = 0; u < QS; ++u) {
-        m[u] = -INFINITY;
-        l[u] = 0.f;
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t) o[u][t] = zero16();
-    }
-
     Stage<TY, DP, C::BK, C::NT> sk, sv;
     unsigned char pb[(C::BK + 63) / 64];
     const auto fetch = [&](int key) {
-        sk.load(tid, a.D, [&](int r) { return key + r < kend ? kp + (int64_t)(key + r) * a.k_l * T::ES : nullptr; });
-        sv.load(tid, a.D, [&](int r) { return key + r < kend ? vp + (int64_t)(key + r) * a.v_l * T::ES : nullptr; });
+        sk.load(tid, a.D, kp + key * a.k_l * T::ES, a.k_l * T::ES, kend - key);
+        sv.load(tid, a.D, vp + key * a.v_l * T::ES, a.v_l * T::ES, kend - key);
 #pragma unroll
         for (int i = 0; i < (C::BK + 63) / 64; ++i) {
             const int j = key + 64 * i + lane;
-            pb[i] = j < kend ? (pad ? pad[j] : 0) : 1;
+            pb[i] = 64 * i + lane < C::BK && j < kend ? (pad ? pad[j] : 0) : 1;
         }
     };
     if (k0 < kend) fetch(k0);
+
+    const int row = tile * C::ROWS + (KEYW ? 0 : 32 * w) + (lane & 31);
+    Frag<T::PL> qf[DP / 16];
+    load_row<TY, DP>(row < a.R ? (const char*)a.q + row_at(a, bh, row, a.q_b, a.q_l, a.q_h) * T::ES : nullptr, a.D, lane, qf);
+    f32x16 o[DP / 32];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) o[t] = zero16();
+
+    int buf = 0;
     for (int key = k0; key < kend; key += C::BK) {
         unsigned long long word[(C::BK + 63) / 64];                        // bit j: key j of the tile takes part
+        bool all = true;
 #pragma unroll
-        for (int i = 0; i < (C::BK + 63) / 64; ++i) word[i] = __builtin_amdgcn_ballot_w64(pb[i] == 0);
-        const auto keep = [&](int r) { return (bool)((C::BK > 64 && r >= 64 ? word[(C::BK + 63) / 64 - 1] >> (r - 64) : word[0] >> (r & 63)) & 1ull); };
-        __syncthreads();
-        sk.store(kt, tid, keep);
-        sv.store(vt, tid, keep);
+        for (int i = 0; i < (C::BK + 63) / 64; ++i) {
+            word[i] = __builtin_amdgcn_ballot_w64(pb[i] == 0);
+            all = all && word[i] == all_keys<C::BK>();
+        }
+        short* const kt = lds + buf * 2 * C::TILE;
+        short* const vt = kt + C::TILE;
+        float* const bi = bias + buf * C::BK;
+        if (C::BUFS == 1) __syncthreads();
+        if (!all) {
+            const auto keep = [&](int r) { return (bool)((C::BK > 64 && r >= 64 ? word[(C::BK + 63) / 64 - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
+            sk.blank(tid, keep);
+            sv.blank(tid, keep);
+            if (tid < C::BK) bi[tid] = keep(tid) ? 0.f : -INFINITY;
+        }
+        sk.store(kt, tid);
+        sv.store(vt, tid);
         __syncthreads();
         if (key + C::BK < kend) fetch(key + C::BK);
+        if (C::BUFS == 2) buf ^= 1;
 
         const int sub0 = KEYW ? w : 0;                                     // this wave's first group of 32 keys
-        f32x16 s[QS][C::KS];
+        if (KEYW && w >= C::NW) continue;
+        f32x16 s[C::KS];
+#pragma unroll
+        for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK>(kt, 32 * (sub0 + t), qf, all, bi + 32 * (sub0 + t), lane);
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < C::KS; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+        mx = fmaxf(mx, other_half(mx));
+        if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > LAZY)) {          // some row of this wave outgrew its maximum
+            const float to = fmaxf(m, mx), f = to > m ? exp2_f((m - to) * a.c) : 1.f;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= f;
+            m = to;
+        }
+        const float sh = T::FSHIFT - (m == -INFINITY ? 0.f : m * a.c);
+        Frag<T::PL> pf[2 * C::KS];
 #pragma unroll
         for (int t = 0; t < C::KS; ++t) {
+            float p[16];
 #pragma unroll
-            for (int u = 0; u < QS; ++u) s[u][t] = zero16();
-#pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                const Frag<T::PL> kf = row_frag<TY, DP, C::BK>(kt, 32 * (sub0 + t), 16 * d, lane);
-#pragma unroll
-                for (int u = 0; u < QS; ++u) s[u][t] = mma<TY>(kf, qf[u][d], s[u][t]);
+            for (int i = 0; i < 16; ++i) {
+                p[i] = exp2_f(fmaf(s[t][i], a.c, sh));
+                l += p[i];
             }
-            const unsigned wd = (unsigned)(word[(sub0 + t) >> 1] >> (32 * ((sub0 + t) & 1)));
-            if (wd != 0xffffffffu) {
-                const unsigned mine = wd >> (4 * half);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int u = 0; u < QS; ++u) s[u][t][i] = mine >> (8 * (i >> 2) + (i & 3)) & 1u ? s[u][t][i] : -INFINITY;
-            }
-        }
-        Frag<T::PL> pf[QS][2 * C::KS];
-#pragma unroll
-        for (int u = 0; u < QS; ++u) {
-            float mx = s[u][0][0];
-#pragma unroll
-            for (int t = 0; t < C::KS; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][t][i]);
-            mx = fmaxf(m[u], fmaxf(mx, other_half(mx)));
-            if (__builtin_amdgcn_ballot_w64(mx > m[u])) {                  // the running maximum grew somewhere in this wave
-                const float f = mx > m[u] ? exp2_f((m[u] - mx) * a.c) : 1.f;
-                l[u] *= f;
-#pragma unroll
-                for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[u][t][i] *= f;
-                m[u] = mx;
-            }
-            const float sh = T::PSHIFT - (m[u] == -INFINITY ? 0.f : m[u] * a.c);
-#pragma unroll
-            for (int t = 0; t < C::KS; ++t) {
-                float p[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    p[i] = exp2_f(fmaf(s[u][t][i], a.c, sh));
-                    l[u] += p[i];
-                }
-                pf[u][2 * t] = make_frag<TY>(p);
-                pf[u][2 * t + 1] = make_frag<TY>(p + 8);
-            }
+            pf[2 * t] = make_frag<TY>(p);
+            pf[2 * t + 1] = make_frag<TY>(p + 8);
         }
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-            for (int j = 0; j < 2 * C::KS; ++j) {
-                const Frag<T::PL> vf = col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16 * j, 32 * t, lane);
-#pragma unroll
-                for (int u = 0; u < QS; ++u) o[u][t] = mma<TY>(vf, pf[u][j], o[u][t]);
-            }
+            for (int j = 0; j < 2 * C::KS; ++j) o[t] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16 * j, 32 * t, lane), pf[j], o[t]);
     }
 
+    const float lt = l + other_half(l);
     if constexpr (KEYW) {
         // join the waves: row statistics first, then each wave's scaled accumulators through LDS
-        float lt = l[0] + other_half(l[0]);
-        if (half == 0) {
-            stat[w * 32 + lane] = m[0];
+        if (half == 0 && w < C::NW) {
+            stat[w * 32 + lane] = m;
             stat[(C::NW + w) * 32 + lane] = lt;
         }
         __syncthreads();                                                    // also: every wave is done with the tiles
@@ -417,18 +476,19 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, QS, KEYW>::NT)) void fwd_kernel(con
             const float x = stat[i * 32 + (lane & 31)];
             L += x == -INFINITY ? 0.f : exp2_f((x - mr) * a.c) * stat[(C::NW + i) * 32 + (lane & 31)];
         }
-        const float f = m[0] == -INFINITY ? 0.f : exp2_f((m[0] - mr) * a.c);
+        const float f = m == -INFINITY ? 0.f : exp2_f((m - mr) * a.c);
         const float inv = L == 0.f ? 0.f : f / L;
         float* acc = reinterpret_cast<float*>(lds);
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[(w * DP + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3)) * 32 + (lane & 31)] = o[0][t][i] * inv;
+            for (int i = 0; i < 16; ++i)
+                if (w < C::NW) acc[(w * DP + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3)) * 32 + (lane & 31)] = o[t][i] * inv;
         __syncthreads();
-        if (w == 0 && half == 0 && row[0] < a.R) {
-            const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L) - T::PSHIFT);
-            if (a.nsplit > 1) a.part_lse[((int64_t)split * a.B * a.Hkv + bh) * a.R + row[0]] = ls;
-            else if (a.lse) a.lse[(int64_t)bh * a.R + row[0]] = L == 0.f ? INFINITY : ls;
+        if (w == 0 && half == 0 && row < a.R) {
+            const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L) - T::FSHIFT);
+            if (a.nsplit > 1) a.part_lse[((int64_t)split * a.B * a.Hkv + bh) * a.R + row] = ls;
+            else if (a.lse) a.lse[(int64_t)bh * a.R + row] = L == 0.f ? INFINITY : ls;
         }
         const int nq = a.D / 4;
         for (int e = tid; e < 32 * nq; e += C::NT) {
@@ -448,34 +508,29 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, QS, KEYW>::NT)) void fwd_kernel(con
             }
         }
     } else {
-#pragma unroll
-        for (int u = 0; u < QS; ++u) {
-            const float L = l[u] + other_half(l[u]);
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            if (row[u] >= a.R) continue;
-            const float ls = L == 0.f ? -INFINITY : m[u] * a.c + (__builtin_amdgcn_logf(L) - T::PSHIFT);
-            const int64_t flat = ((int64_t)split * a.B * a.Hkv + bh) * a.R + row[u];
-            if (half == 0) {
-                if (a.nsplit > 1) a.part_lse[flat] = ls;
-                else if (a.lse) a.lse[(int64_t)bh * a.R + row[u]] = L == 0.f ? INFINITY : ls;
-            }
-            const int64_t at = a.nsplit > 1 ? flat * a.D : out_at(a, bh, row[u]);
-#pragma unroll
-            for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int d = 32 * t + 8 * g;
-                    if (d >= a.D) continue;
-                    const float x0 = o[u][t][4 * g] * inv, x1 = o[u][t][4 * g + 1] * inv, x2 = o[u][t][4 * g + 2] * inv,
-                                x3 = o[u][t][4 * g + 3] * inv;
-                    if (a.nsplit > 1) {
-                        put4<F32>(a.part, at + d + 4 * half, x0, x1, x2, x3);
-                    } else {
-                        put4<TY>(a.o, at + d + 4 * half, x0, x1, x2, x3);
-                        if (a.o32) put4<F32>(a.o32, at + d + 4 * half, x0, x1, x2, x3);
-                    }
-                }
+        if (row >= a.R) return;
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        const float ls = lt == 0.f ? -INFINITY : m * a.c + (__builtin_amdgcn_logf(lt) - T::FSHIFT);
+        const int64_t flat = ((int64_t)split * a.B * a.Hkv + bh) * a.R + row;
+        if (half == 0) {
+            if (a.nsplit > 1) a.part_lse[flat] = ls;
+            else if (a.lse) a.lse[(int64_t)bh * a.R + row] = lt == 0.f ? INFINITY : ls;
         }
+        const int64_t at = a.nsplit > 1 ? flat * a.D : out_at(a, bh, row);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * t + 8 * g;
+                if (d >= a.D) continue;
+                const float x0 = o[t][4 * g] * inv, x1 = o[t][4 * g + 1] * inv, x2 = o[t][4 * g + 2] * inv, x3 = o[t][4 * g + 3] * inv;
+                if (a.nsplit > 1) {
+                    put4<F32>(a.part, at + d + 4 * half, x0, x1, x2, x3);
+                } else {
+                    put4<TY>(a.o, at + d + 4 * half, x0, x1, x2, x3);
+                    if (a.o32) put4<F32>(a.o32, at + d + 4 * half, x0, x1, x2, x3);
+                }
+            }
     }
 }
 
@@ -514,19 +569,20 @@ template <int TY, int NACC> struct DsScale {
 // transposed as in the forward pass (K and V rows are A operands), dq^T accumulates K^T ds^T.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DqCfg {
-    static constexpr int BK = 64, NT = 256, ROWS = 128;
+    static constexpr int BK = TY == F32 ? 32 : 64, NT = 256, ROWS = 128;
+    static constexpr int WAVES = TY == F32 && DP > 64 ? 1 : 2;
     static constexpr int TILE = tile_len<TY, DP, BK>();
-    static constexpr size_t LDS = 2 * TILE * 2 + 16;
+    static constexpr int BUFS = bufs_of(TILE, WAVES);
+    static constexpr size_t LDS = 2 * TILE * BUFS * 2 + BUFS * BK * 4 + 16;
 };
 
 template <int TY, int DP>
-__global__ __launch_bounds__(256) void bwd_dq_kernel(const Args a) {
+__global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(const Args a) {
     using C = DqCfg<TY, DP>;
     using T = Ty<TY>;
     extern __shared__ __attribute__((aligned(16))) short lds[];
-    short* const kt = lds;
-    short* const vt = lds + C::TILE;
-    int* const red = reinterpret_cast<int*>(lds + 2 * C::TILE);
+    float* const bias = reinterpret_cast<float*>(lds + 2 * C::TILE * C::BUFS);
+    int* const red = reinterpret_cast<int*>(bias + C::BUFS * C::BK);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tile = id % a.tiles; id /= a.tiles;
@@ -537,24 +593,29 @@ __global__ __launch_bounds__(256) void bwd_dq_kernel(const Args a) {
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
     const int k0 = split * a.span, kend = last_key<C::NT>(pad, k0, min(a.Lk, k0 + a.span), tid, red);
 
+    Stage<TY, DP, C::BK, C::NT> sk, sv;
+    unsigned char pb;
+    const auto fetch = [&](int key) {
+        sk.load(tid, a.D, kp + key * a.k_l * T::ES, a.k_l * T::ES, kend - key);
+        sv.load(tid, a.D, vp + key * a.v_l * T::ES, a.v_l * T::ES, kend - key);
+        const int j = key + lane;
+        pb = lane < C::BK && j < kend ? (pad ? pad[j] : 0) : 1;
+    };
+    if (k0 < kend) fetch(k0);
+
     const int row = tile * C::ROWS + 32 * w + (lane & 31);
     const bool in = row < a.R;
     Frag<T::PL> qf[DP / 16], df[DP / 16];
+    load_row<TY, DP>(in ? (const char*)a.q + row_at(a, bh, row, a.q_b, a.q_l, a.q_h) * T::ES : nullptr, a.D, lane, qf);
+    load_row<TY, DP>(in ? (const char*)a.dout + row_at(a, bh, row, a.d_b, a.d_l, a.d_h) * T::ES : nullptr, a.D, lane, df);
     float delta = 0.f;
     {
-        float f[DP / 16][8];
-        load_row<TY, DP>(in ? (const char*)a.q + row_at(a, bh, row, a.q_b, a.q_l, a.q_h) * T::ES : nullptr, a.D, lane, f);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) qf[s] = make_frag<TY>(f[s]);
         float g[DP / 16][8];
-        load_row<TY, DP>(in ? (const char*)a.dout + row_at(a, bh, row, a.d_b, a.d_l, a.d_h) * T::ES : nullptr, a.D, lane, f);
-        load_row<F32, DP>(in ? a.o32 + out_at(a, bh, row) : nullptr, a.D, lane, g);
+        load_floats<DP>(in ? a.o32 + out_at(a, bh, row) : nullptr, a.D, lane, g);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-            df[s] = make_frag<TY>(f[s]);
+        for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) delta = fmaf(f[s][j], g[s][j], delta);
-        }
+            for (int j = 0; j < 8; ++j) delta = fmaf(frag_at<TY>(df[s], j), g[s][j], delta);
         delta += other_half(delta);
     }
     const float ls = (in ? a.lse[(int64_t)bh * a.R + row] : INFINITY) - T::PSHIFT;
@@ -564,44 +625,35 @@ __global__ __launch_bounds__(256) void bwd_dq_kernel(const Args a) {
     for (int t = 0; t < DP / 32; ++t) acc[t] = zero16();
     DsScale<TY, DP / 32> sc;
 
-    Stage<TY, DP, C::BK, C::NT> sk, sv;
-    unsigned char pb;
-    const auto fetch = [&](int key) {
-        sk.load(tid, a.D, [&](int r) { return key + r < kend ? kp + (int64_t)(key + r) * a.k_l * T::ES : nullptr; });
-        sv.load(tid, a.D, [&](int r) { return key + r < kend ? vp + (int64_t)(key + r) * a.v_l * T::ES : nullptr; });
-        const int j = key + lane;
-        pb = j < kend ? (pad ? pad[j] : 0) : 1;
-    };
-    if (k0 < kend) fetch(k0);
+    int buf = 0;
     for (int key = k0; key < kend; key += C::BK) {
         const unsigned long long word = __builtin_amdgcn_ballot_w64(pb == 0);
-        const auto keep = [&](int r) { return (bool)(word >> r & 1ull); };
-        __syncthreads();
-        sk.store(kt, tid, keep);
-        sv.store(vt, tid, keep);
+        const bool all = word == all_keys<C::BK>();
+        short* const kt = lds + buf * 2 * C::TILE;
+        short* const vt = kt + C::TILE;
+        float* const bi = bias + buf * C::BK;
+        if (C::BUFS == 1) __syncthreads();
+        if (!all) {
+            const auto keep = [&](int r) { return (bool)(word >> r & 1ull); };
+            sk.blank(tid, keep);
+            sv.blank(tid, keep);
+            if (tid < C::BK) bi[tid] = keep(tid) ? 0.f : -INFINITY;
+        }
+        sk.store(kt, tid);
+        sv.store(vt, tid);
         __syncthreads();
         if (key + C::BK < kend) fetch(key + C::BK);
+        if (C::BUFS == 2) buf ^= 1;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const unsigned wd = (unsigned)(word >> (32 * t));
-            if (wd == 0) continue;
-            f32x16 s = zero16(), dp = zero16();
+        for (int t = 0; t < C::BK / 32; ++t) {
+            if ((unsigned)(word >> (32 * t)) == 0) continue;
+            const f32x16 s = scores<TY, DP, C::BK>(kt, 32 * t, qf, all, bi + 32 * t, lane);
+            f32x16 dp = zero16();
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                s = mma<TY>(row_frag<TY, DP, C::BK>(kt, 32 * t, 16 * d, lane), qf[d], s);
-                dp = mma<TY>(row_frag<TY, DP, C::BK>(vt, 32 * t, 16 * d, lane), df[d], dp);
-            }
+            for (int d = 0; d < DP / 16; ++d) dp = mma<TY>(row_frag<TY, DP, C::BK>(vt, 32 * t, 16 * d, lane), df[d], dp);
             float ds[16];
-            const unsigned mine = wd >> (4 * half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = exp2_f(fmaf(s[i], a.c, -ls));
-                ds[i] = p * (dp[i] - delta);
-            }
-            if (wd != 0xffffffffu) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) ds[i] = mine >> (8 * (i >> 2) + (i & 3)) & 1u ? ds[i] : 0.f;
-            }
+            for (int i = 0; i < 16; ++i) ds[i] = exp2_f(fmaf(s[i], a.c, -ls)) * (dp[i] - delta);
             sc.fit(ds, acc);
             const Frag<T::PL> f0 = make_frag<TY>(ds), f1 = make_frag<TY>(ds + 8);
 #pragma unroll
@@ -631,19 +683,19 @@ __global__ __launch_bounds__(256) void bwd_dq_kernel(const Args a) {
 // lane owns a KEY: dk^T += Q^T ds, dv^T += dO^T p.  A padded key's column touches no other, so its result is simply written as zeros.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DkvCfg {
-    static constexpr int BR = 64, NT = 256, KEYS = 128;
+    static constexpr int BR = TY == F32 || DP > 64 ? 32 : 64, NT = 256, KEYS = 128;
+    static constexpr int WAVES = (TY == F32 && DP > 32) || DP == 128 ? 1 : 2;
     static constexpr int TILE = tile_len<TY, DP, BR>();
-    static constexpr size_t LDS = 2 * TILE * 2 + 2 * BR * 4 + 16;
+    static constexpr int BUFS = bufs_of(TILE, WAVES);
+    static constexpr size_t LDS = 2 * TILE * BUFS * 2 + BUFS * 2 * BR * 4;
 };
 
 template <int TY, int DP>
-__global__ __launch_bounds__(256) void bwd_dkv_kernel(const Args a) {
+__global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(const Args a) {
     using C = DkvCfg<TY, DP>;
     using T = Ty<TY>;
     extern __shared__ __attribute__((aligned(16))) short lds[];
-    short* const qt = lds;
-    short* const dt = lds + C::TILE;
-    float* const lsd = reinterpret_cast<float*>(lds + 2 * C::TILE);        // [64] log-sums, [64] deltas of the tile's rows
+    float* const stat = reinterpret_cast<float*>(lds + 2 * C::TILE * C::BUFS);    // [BUFS][BR log-sums, BR deltas] of the tile's rows
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tile = id % a.tiles; id /= a.tiles;
@@ -654,75 +706,85 @@ __global__ __launch_bounds__(256) void bwd_dkv_kernel(const Args a) {
     const bool work = __builtin_amdgcn_ballot_w64(live) != 0;             // of this wave
     const int r0 = split * a.span, rend = __syncthreads_or(work) ? min(a.R, r0 + a.span) : r0;
 
-    Frag<T::PL> kf[DP / 16], vf[DP / 16];
-    {
-        float f[DP / 16][8];
-        load_row<TY, DP>(live ? (const char*)a.k + (b * a.k_b + key * a.k_l + kv * a.k_h) * T::ES : nullptr, a.D, lane, f);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) kf[s] = make_frag<TY>(f[s]);
-        load_row<TY, DP>(live ? (const char*)a.v + (b * a.v_b + key * a.v_l + kv * a.v_h) * T::ES : nullptr, a.D, lane, f);
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) vf[s] = make_frag<TY>(f[s]);
-    }
-    f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
-    DsScale<TY, DP / 32> sc;
-
     Stage<TY, DP, C::BR, C::NT> sq, sd;
     float st = 0.f;
     const char* const qb = (const char*)a.q + (b * a.q_b + (int64_t)kv * a.G * a.q_h) * T::ES;
     const char* const db = (const char*)a.dout + (b * a.d_b + (int64_t)kv * a.G * a.d_h) * T::ES;
     const auto fetch = [&](int r) {
-        const int g0 = r / a.Lq, i0 = r - g0 * a.Lq;                       // uniform
-        const auto at = [&](int x, const char* base, int64_t sl, int64_t sh) -> const char* {
-            if (r + x >= rend) return nullptr;
-            int g = g0, i = i0 + x;
-            if (i >= a.Lq) { g += i / a.Lq; i %= a.Lq; }
-            return base + (i * sl + g * sh) * T::ES;
-        };
-        sq.load(tid, a.D, [&](int x) { return at(x, qb, a.q_l, a.q_h); });
-        sd.load(tid, a.D, [&](int x) { return at(x, db, a.d_l, a.d_h); });
-        const int x = r + (tid & 63);
-        if (tid < 64) st = x < rend ? a.lse[(int64_t)bh * a.R + x] - T::PSHIFT : INFINITY;
-        else if (tid < 128) st = x < rend ? a.delta[(int64_t)bh * a.R + x] : 0.f;
+        const int g0 = r / a.Lq, i0 = r - g0 * a.Lq, here = min(rend - r, a.Lq - i0);      // rows of head g0 from here on
+        if (here >= min(rend - r, C::BR)) {                                // the tile's rows are of one head
+            sq.load(tid, a.D, qb + (i0 * a.q_l + g0 * a.q_h) * T::ES, a.q_l * T::ES, here);
+            sd.load(tid, a.D, db + (i0 * a.d_l + g0 * a.d_h) * T::ES, a.d_l * T::ES, here);
+        } else {
+            const auto at = [&](int x, const char* base, int64_t sl, int64_t sh) -> const char* {
+                if (r + x >= rend) return nullptr;
+                const int g = (r + x) / a.Lq, i = r + x - g * a.Lq;
+                return base + (i * sl + g * sh) * T::ES;
+            };
+            sq.gather(tid, a.D, [&](int x) { return at(x, qb, a.q_l, a.q_h); });
+            sd.gather(tid, a.D, [&](int x) { return at(x, db, a.d_l, a.d_h); });
+        }
+        const int x = r + tid % C::BR;
+        if (tid < C::BR) st = x < rend ? a.lse[(int64_t)bh * a.R + x] - T::PSHIFT : INFINITY;
+        else if (tid < 2 * C::BR) st = x < rend ? a.delta[(int64_t)bh * a.R + x] : 0.f;
     };
     if (r0 < rend) fetch(r0);
+
+    Frag<T::PL> kf[DP / 16], vf[DP / 16];
+    load_row<TY, DP>(live ? (const char*)a.k + (b * a.k_b + key * a.k_l + kv * a.k_h) * T::ES : nullptr, a.D, lane, kf);
+    load_row<TY, DP>(live ? (const char*)a.v + (b * a.v_b + key * a.v_l + kv * a.v_h) * T::ES : nullptr, a.D, lane, vf);
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
+    DsScale<TY, DP / 32> sc;
+
+    int buf = 0;
     for (int r = r0; r < rend; r += C::BR) {
-        __syncthreads();
-        sq.store(qt, tid, [](int) { return true; });
-        sd.store(dt, tid, [](int) { return true; });
-        if (tid < 128) lsd[tid] = st;
+        short* const qt = lds + buf * 2 * C::TILE;
+        short* const dt = qt + C::TILE;
+        float* const lsd = stat + buf * 2 * C::BR;
+        if (C::BUFS == 1) __syncthreads();
+        sq.store(qt, tid);
+        sd.store(dt, tid);
+        if (tid < 2 * C::BR) lsd[tid] = st;
         __syncthreads();
         if (r + C::BR < rend) fetch(r + C::BR);
+        if (C::BUFS == 2) buf ^= 1;
         if (!work) continue;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < C::BR / 32; ++t) {
             if (r + 32 * t >= rend) continue;
             f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                s = mma<TY>(row_frag<TY, DP, C::BR>(qt, 32 * t, 16 * d, lane), kf[d], s);
-                dp = mma<TY>(row_frag<TY, DP, C::BR>(dt, 32 * t, 16 * d, lane), vf[d], dp);
-            }
-            float p[16], ds[16];
+            for (int d = 0; d < DP / 16; ++d) s = mma<TY>(row_frag<TY, DP, C::BR>(qt, 32 * t, 16 * d, lane), kf[d], s);
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) dp = mma<TY>(row_frag<TY, DP, C::BR>(dt, 32 * t, 16 * d, lane), vf[d], dp);
+            float p[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const fx4 ls = *reinterpret_cast<const fx4*>(lsd + 32 * t + 8 * g + 4 * half);
-                const fx4 de = *reinterpret_cast<const fx4*>(lsd + 64 + 32 * t + 8 * g + 4 * half);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[4 * g + i] = exp2_f(fmaf(s[4 * g + i], a.c, -ls[i]));
-                    ds[4 * g + i] = p[4 * g + i] * (dp[4 * g + i] - de[i]);
+                for (int i = 0; i < 4; ++i) p[4 * g + i] = exp2_f(fmaf(s[4 * g + i], a.c, -ls[i]));
+            }
+            {
+                const Frag<T::PL> p0 = make_frag<TY>(p), p1 = make_frag<TY>(p + 8);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    dv[d] = mma<TY>(col_frag<TY, DP, C::BR>(dt, 32 * t, 32 * d, lane), p0, dv[d]);
+                    dv[d] = mma<TY>(col_frag<TY, DP, C::BR>(dt, 32 * t + 16, 32 * d, lane), p1, dv[d]);
                 }
             }
-            sc.fit(ds, dk);
-            const Frag<T::PL> p0 = make_frag<TY>(p), p1 = make_frag<TY>(p + 8), d0 = make_frag<TY>(ds), d1 = make_frag<TY>(ds + 8);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const fx4 de = *reinterpret_cast<const fx4*>(lsd + C::BR + 32 * t + 8 * g + 4 * half);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[4 * g + i] *= dp[4 * g + i] - de[i];
+            }
+            sc.fit(p, dk);
+            const Frag<T::PL> d0 = make_frag<TY>(p), d1 = make_frag<TY>(p + 8);
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) {
-                dv[d] = mma<TY>(col_frag<TY, DP, C::BR>(dt, 32 * t, 32 * d, lane), p0, dv[d]);
                 dk[d] = mma<TY>(col_frag<TY, DP, C::BR>(qt, 32 * t, 32 * d, lane), d0, dk[d]);
-                dv[d] = mma<TY>(col_frag<TY, DP, C::BR>(dt, 32 * t + 16, 32 * d, lane), p1, dv[d]);
                 dk[d] = mma<TY>(col_frag<TY, DP, C::BR>(qt, 32 * t + 16, 32 * d, lane), d1, dk[d]);
             }
         }
@@ -753,27 +815,46 @@ __global__ __launch_bounds__(256) void bwd_dkv_kernel(const Args a) {
 }
 
 // ---- joining splits -------------------------------------------------------------------------------------------------------------------
-// forward: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max); a thread owns four columns of a row
+// forward: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  A workgroup owns a row: its threads take four columns of every
+// (256 / columns)-th split, so that one latency covers many splits, and are summed in a fixed order.
+constexpr int MOST_SPLITS = 1024;
+
 template <int TY>
 __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
-    const int nq = a.D / 4;
-    const int64_t rows = (int64_t)a.B * a.Hkv * a.R, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= rows * nq) return;
-    const int64_t fr = e / nq;
-    const int d = 4 * (int)(e % nq);
+    __shared__ float wgt[MOST_SPLITS], part[256][4], red[8];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int64_t rows = (int64_t)a.B * a.Hkv * a.R, fr = blockIdx.x;
     float M = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, a.part_lse[s * rows + fr]);
+    for (int s = tid; s < a.nsplit; s += 256) M = fmaxf(M, wgt[s] = a.part_lse[s * rows + fr]);
+    M = wave_max(M);
+    if (lane == 0) red[w] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float mr = M == -INFINITY ? 0.f : M;
     float W = 0.f;
-    fx4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float wgt = exp2_f(a.part_lse[s * rows + fr] - mr);
-        const fx4 y = *reinterpret_cast<const fx4*>(a.part + (s * rows + fr) * a.D + d);
-        W += wgt;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = fmaf(wgt, y[j], x[j]);
-    }
+    for (int s = tid; s < a.nsplit; s += 256) W += wgt[s] = exp2_f(wgt[s] - mr);
+    W = wave_sum(W);
+    if (lane == 0) red[4 + w] = W;
+    __syncthreads();
+    W = red[4] + red[5] + red[6] + red[7];
     const float inv = W == 0.f ? 0.f : 1.f / W;
+    const int nq = a.D / 4, ng = 256 / nq, g = tid / nq, d = 4 * (tid % nq);
+    fx4 x = {0.f, 0.f, 0.f, 0.f};
+    if (g < ng)
+        for (int s = g; s < a.nsplit; s += ng) {
+            const fx4 y = *reinterpret_cast<const fx4*>(a.part + (s * rows + fr) * a.D + d);
+            const float f = wgt[s];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = fmaf(f, y[j], x[j]);
+        }
+    *reinterpret_cast<fx4*>(part[tid]) = x;
+    __syncthreads();
+    if (g) return;
+    for (int i = 1; i < ng; ++i) {
+        const fx4 y = *reinterpret_cast<const fx4*>(part[i * nq + tid]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += y[j];
+    }
     const int bh = (int)(fr / a.R), r = (int)(fr % a.R);
     const int64_t at = out_at(a, bh, r) + d;
     put4<TY>(a.o, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
@@ -795,7 +876,7 @@ __global__ __launch_bounds__(256) void join_sum_kernel(const float* part, void* 
 }
 
 // ---- launches of one element type (defined in that type's unit) -------------------------------------------------------------------------
-template <int TY> int launch_fwd(const Args& a, int keyw, int qs, hipStream_t s);
+template <int TY> int launch_fwd(const Args& a, int keyw, hipStream_t s);
 template <int TY> int launch_join_fwd(const Args& a, hipStream_t s);
 template <int TY> int launch_bwd_dq(const Args& a, hipStream_t s);
 template <int TY> int launch_bwd_dkv(const Args& a, hipStream_t s);

@@ -7,7 +7,7 @@ using namespace xattn;
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 struct Plan {
-    int keyw, qs, tiles, nsplit, span;
+    int keyw, tiles, nsplit, span;
 };
 
 // Splits the streamed axis (n elements, steps of `step`, no span under `least`) until about `want` workgroups run.
@@ -15,6 +15,7 @@ void split_axis(int64_t base, int64_t n, int step, int least, int64_t want, Plan
     int64_t s = base >= want ? 1 : (want + base - 1) / base;
     const int64_t most = n / least > 1 ? n / least : 1;
     if (s > most) s = most;
+    if (s > MOST_SPLITS) s = MOST_SPLITS;
     const int64_t span = up((n + s - 1) / s, step);
     p.span = (int)span;
     p.nsplit = (int)((n + span - 1) / span);
@@ -26,14 +27,12 @@ Plan plan_fwd(const favae_xattn_desc* d) {
     const int64_t R = (int64_t)d->H / d->Hkv * d->Lq, heads = (int64_t)d->B * d->Hkv;
     const bool f32 = d->dtype == F32;
     Plan p{};
-    p.qs = 1;
     if (R <= 64) {
         p.keyw = 1;
         p.tiles = (int)((R + 31) / 32);
         split_axis(p.tiles * heads, d->Lk, f32 && dim_pad(d->D) > 64 ? 64 : 128, 256, 1024, p);
     } else {
-        if (!f32 && d->D <= 64 && (R + 255) / 256 * heads >= 512) p.qs = 2;
-        p.tiles = (int)((R + 128 * p.qs - 1) / (128 * p.qs));
+        p.tiles = (int)((R + 127) / 128);
         split_axis(p.tiles * heads, d->Lk, 64, 512, 512, p);
     }
     return p;
@@ -64,6 +63,8 @@ bool ok_desc(const favae_xattn_desc* d) {
     const int64_t unit = d->dtype == F32 ? 4 : 8;                          // 16-byte accesses
     for (int64_t s : {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh})
         if (s < 0 || s % unit) return false;
+    for (int64_t s : {d->q_sl, d->k_sl, d->v_sl})                          // rows follow one another and 128 of them span less than 2^31 bytes
+        if (s < d->D || s * (16 / unit) >= (1 << 24)) return false;
     return true;
 }
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -86,7 +87,7 @@ void use(Args& a, const Plan& p) { a.tiles = p.tiles; a.nsplit = p.nsplit; a.spa
 int64_t rows_of(const favae_xattn_desc* d) { return (int64_t)d->B * d->H * d->Lq; }
 
 int run_fwd(int ty, const Args& a, const Plan& p, hipStream_t s) {
-    return ty == F32 ? launch_fwd<F32>(a, p.keyw, p.qs, s) : ty == BF16 ? launch_fwd<BF16>(a, p.keyw, p.qs, s) : launch_fwd<F16>(a, p.keyw, p.qs, s);
+    return ty == F32 ? launch_fwd<F32>(a, p.keyw, s) : ty == BF16 ? launch_fwd<BF16>(a, p.keyw, s) : launch_fwd<F16>(a, p.keyw, s);
 }
 int run_join_fwd(int ty, const Args& a, hipStream_t s) {
     return ty == F32 ? launch_join_fwd<F32>(a, s) : ty == BF16 ? launch_join_fwd<BF16>(a, s) : launch_join_fwd<F16>(a, s);

@@ -11,22 +11,16 @@ inline int ready(F kern, size_t lds) {
                ? FAVAE_OK : favae_prof_fail_(FAVAE_ERR_LAUNCH);
 }
 
-template <int TY, int DP, int QS, bool KEYW>
+template <int TY, int DP, bool KEYW>
 int go_fwd(const Args& a, hipStream_t s) {
-    using C = FwdCfg<TY, DP, QS, KEYW>;
-    if (int rc = ready(fwd_kernel<TY, DP, QS, KEYW>, C::LDS)) return rc;
-    FAVAE_KLAUNCH((fwd_kernel<TY, DP, QS, KEYW>), dim3((unsigned)(a.tiles * a.nsplit) * a.B * a.Hkv), dim3(C::NT), C::LDS, s, a);
+    using C = FwdCfg<TY, DP, KEYW>;
+    if (int rc = ready(fwd_kernel<TY, DP, KEYW>, C::LDS)) return rc;
+    FAVAE_KLAUNCH((fwd_kernel<TY, DP, KEYW>), dim3((unsigned)(a.tiles * a.nsplit) * a.B * a.Hkv), dim3(C::NT), C::LDS, s, a);
     FAVAE_CHECK_LAUNCH();
     return FAVAE_OK;
 }
 template <int TY, int DP>
-int go_fwd_dp(const Args& a, int keyw, int qs, hipStream_t s) {
-    if (keyw) return go_fwd<TY, DP, 1, true>(a, s);
-    if constexpr (TY != F32 && DP <= 64) {
-        if (qs == 2) return go_fwd<TY, DP, 2, false>(a, s);
-    }
-    return go_fwd<TY, DP, 1, false>(a, s);
-}
+int go_fwd_dp(const Args& a, int keyw, hipStream_t s) { return keyw ? go_fwd<TY, DP, true>(a, s) : go_fwd<TY, DP, false>(a, s); }
 template <int TY, int DP>
 int go_dq(const Args& a, hipStream_t s) {
     using C = DqCfg<TY, DP>;
@@ -44,9 +38,9 @@ int go_dkv(const Args& a, hipStream_t s) {
     return FAVAE_OK;
 }
 
-template <int TY> int launch_fwd(const Args& a, int keyw, int qs, hipStream_t s) {
-    return a.D <= 32 ? go_fwd_dp<TY, 32>(a, keyw, qs, s) : a.D <= 64 ? go_fwd_dp<TY, 64>(a, keyw, qs, s)
-         : a.D <= 96 ? go_fwd_dp<TY, 96>(a, keyw, qs, s) : go_fwd_dp<TY, 128>(a, keyw, qs, s);
+template <int TY> int launch_fwd(const Args& a, int keyw, hipStream_t s) {
+    return a.D <= 32 ? go_fwd_dp<TY, 32>(a, keyw, s) : a.D <= 64 ? go_fwd_dp<TY, 64>(a, keyw, s)
+         : a.D <= 96 ? go_fwd_dp<TY, 96>(a, keyw, s) : go_fwd_dp<TY, 128>(a, keyw, s);
 }
 template <int TY> int launch_bwd_dq(const Args& a, hipStream_t s) {
     return a.D <= 32 ? go_dq<TY, 32>(a, s) : a.D <= 64 ? go_dq<TY, 64>(a, s) : a.D <= 96 ? go_dq<TY, 96>(a, s) : go_dq<TY, 128>(a, s);
@@ -55,8 +49,7 @@ template <int TY> int launch_bwd_dkv(const Args& a, hipStream_t s) {
     return a.D <= 32 ? go_dkv<TY, 32>(a, s) : a.D <= 64 ? go_dkv<TY, 64>(a, s) : a.D <= 96 ? go_dkv<TY, 96>(a, s) : go_dkv<TY, 128>(a, s);
 }
 template <int TY> int launch_join_fwd(const Args& a, hipStream_t s) {
-    const int64_t n = (int64_t)a.B * a.Hkv * a.R * (a.D / 4);
-    FAVAE_KLAUNCH((join_fwd_kernel<TY>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    FAVAE_KLAUNCH((join_fwd_kernel<TY>), dim3((unsigned)(a.B * a.Hkv) * a.R), dim3(256), 0, s, a);
     FAVAE_CHECK_LAUNCH();
     return FAVAE_OK;
 }
@@ -68,7 +61,7 @@ template <int TY> int launch_join_sum(const float* part, void* out, int64_t n, i
 
 #define XATTN_INSTANTIATE(TY)                                                                  \
     namespace xattn {                                                                          \
-    template int launch_fwd<TY>(const Args&, int, int, hipStream_t);                           \
+    template int launch_fwd<TY>(const Args&, int, hipStream_t);                           \
     template int launch_bwd_dq<TY>(const Args&, hipStream_t);                                  \
     template int launch_bwd_dkv<TY>(const Args&, hipStream_t);                                 \
     template int launch_join_fwd<TY>(const Args&, hipStream_t);                                \

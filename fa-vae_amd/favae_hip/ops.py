@@ -1889,10 +1889,14 @@ def _dense16(t):
 
 
 def _rows16(t):
-    """(B, L, H, D) with contiguous columns and 16-byte aligned rows (a dense copy where it has not)"""
-    unit = 16 // t.element_size()
+    """(B, L, H, D) with contiguous columns and rows that the kernels can read in place (include/favae_hip.h), else a dense copy"""
+    es = t.element_size()
     sb, sl, sh, sd = t.stride()
-    return t if sd == 1 and not (sb % unit or sl % unit or sh % unit or t.data_ptr() % 16) else t.clone(memory_format=torch.contiguous_format)
+    if t.shape[1] == 1:
+        sl = t.shape[3]
+    if sd == 1 and not ((sb | sl | sh) * es | t.data_ptr()) & 15 and t.shape[3] <= sl < (1 << 24) // es:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1904,7 +1908,15 @@ def _xattn_desc(*fields):
 
 def _xattn_plan(q, k, v, pad, scale):
     B, Lq, H, D = q.shape
-    return _xattn_desc(B, Lq, k.shape[1], H, k.shape[2], D, _DTYPE_ID[q.dtype], scale, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+    Lk = k.shape[1]
+    qb, ql, qh, _ = q.stride()
+    kb, kl, kh, _ = k.stride()
+    vb, vl, vh, _ = v.stride()
+    if Lq == 1:                                           # the stride of an axis of one says nothing
+        ql = D
+    if Lk == 1:
+        kl = vl = D
+    return _xattn_desc(B, Lq, Lk, H, k.shape[2], D, _DTYPE_ID[q.dtype], scale, qb, ql, qh, kb, kl, kh, vb, vl, vh,
                        0 if pad is None else pad.stride(0))
 
 

@@ -105,7 +105,7 @@ def test_c_entry_points_refuse_before_they_launch():
     assert bwd(desc(), dk=None) == bad_arg and bwd(desc(), dv=None) == bad_arg   # both or neither
     for d in (desc(D=36), desc(D=136), desc(D=0), desc(H=7), desc(Hkv=0), desc(B=0), desc(Lq=0), desc(Lk=0), desc(dtype=3), desc(dtype=-1),
               desc(scale=0.0), desc(scale=-1.0), desc(scale=float("inf")), desc(scale=float("nan")), desc(q_sl=260), desc(k_sb=-320),
-              desc(v_sh=4), desc(dtype=0, k_sl=66), desc(Lq=1 << 30)):
+              desc(v_sh=4), desc(dtype=0, k_sl=66), desc(Lq=1 << 30), desc(k_sl=0), desc(v_sl=24), desc(q_sl=1 << 23)):
         assert fwd(d) == unsupported and bwd(d) == unsupported
         assert lib.favae_xattn_fwd_workspace(byref(d)) == 0 and lib.favae_xattn_bwd_workspace(byref(d)) == 0
     assert fwd(desc(), q=P + 8) == unsupported and fwd(desc(), o=P + 4) == unsupported and bwd(desc(), dq=P + 2) == unsupported

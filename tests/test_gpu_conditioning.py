@@ -176,6 +176,8 @@ def test_layouts_are_read_where_they_are(dtype):
     hm = [t.transpose(1, 2).contiguous().requires_grad_() for t in (q0, k0, v0)]  # head-major memory
     got = grads(hm, *(t.transpose(1, 2) for t in hm))
     assert all(torch.equal(a, b) for a, b in zip(got, (ref[0], *(t.transpose(1, 2) for t in ref[1:]))))
+    flat = k0[:, :1].expand(-1, Lk, -1, -1)                                      # a length stride of 0: copied
+    assert torch.equal(K.cross_attention(q0, flat, v0), K.cross_attention(q0, flat.contiguous(), v0))
     big = torch.zeros(B, Lk, H, D + 1, dtype=dt, device=DEV)                     # rows that begin at odd addresses: copied
     big[..., 1:] = k0
     assert torch.equal(K.cross_attention(q0, big[..., 1:], v0), ref[0])
@@ -290,10 +292,11 @@ def test_empty_axes(shape):
     assert all(a.shape == b.shape and not a.any() for a, b in zip(g, (q, k, v)))
 
 
-def test_offsets_beyond_32_bits():
-    """rows of a long cache more than 2^32 bytes (and 2^31 elements) from its start"""
+@pytest.mark.parametrize("Lk, step", [(700, 2 ** 22), (70, 2 ** 25)])
+def test_offsets_beyond_32_bits(Lk, step):
+    """rows of a long cache more than 2^32 bytes (and 2^31 elements) from its start, read in place and (rows very far apart) copied first"""
     K = ops()
-    Lk, D, step = 70, 32, 2 ** 25
+    D = 32
     if torch.cuda.mem_get_info()[0] < 16 << 30:
         pytest.skip("needs 10 GB")
     cache = torch.empty((Lk * step + 2 * D,), dtype=torch.float16, device=DEV)
