@@ -72,38 +72,33 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* ids, const v
     const int n = (int)(T - t0 < rows ? T - t0 : rows) * cpr;
     for (int e0 = threadIdx.x; e0 < n; e0 += 1024) {
         P p[4];
-        int64_t to[4];
+        int64_t id[4];
+        int r[4], c[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int e = e0 + 256 * u;
-            to[u] = -1;
-            if (e < n) {
-                const int r = e / cpr, c = (e - r * cpr) * P::N;
-                const int64_t id = id_at<I>(ids, t0 + r);
-                to[u] = (t0 + r) * C + c;
-                if (id >= 0 && id < V) {
-                    p[u].load(w, id * w_stride + c);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < P::N; ++i) p[u].x[i] = __builtin_nanf("");
-                }
-            }
+        for (int u = 0; u < 4; ++u) {                                      // no branch: the four loads of each kind are in flight together
+            const int e = min(e0 + 256 * u, n - 1);
+            r[u] = e / cpr;
+            c[u] = (e - r[u] * cpr) * P::N;
+            id[u] = id_at<I>(ids, t0 + r[u]);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (to[u] >= 0) {
+        for (int u = 0; u < 4; ++u) p[u].load(w, (id[u] >= 0 && id[u] < V ? id[u] : 0) * w_stride + c[u]);
 #pragma unroll
-                for (int i = 0; i < P::N; ++i) p[u].x[i] *= scale;
-                p[u].store(out, to[u]);
+        for (int u = 0; u < 4; ++u)
+            if (e0 + 256 * u < n) {
+                const bool ok = id[u] >= 0 && id[u] < V;
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) p[u].x[i] = ok ? p[u].x[i] * scale : __builtin_nanf("");
+                p[u].store(out, (t0 + r[u]) * C + c[u]);
             }
     }
 }
 
 // ---- stable sort of (id, t) by id: 8 bits a pass, least significant first -----------------------------------------------------------
-// Block b owns `tpb` consecutive entries.  count[p][digit][block]: how many entries of the block have that digit of pass p.  The counts
-// of pass 0 are written by embed_count_kernel, those of a later pass by atomic adds of the pass before it (an entry knows where it goes;
-// integer counts do not depend on the order).  Ids outside [0, V) and the padding id are left out; *valid = entries that remain.
-constexpr int DIGITS = 256, SORT_BLOCKS = 256, BATCH = 1024;
+// Block b owns `tpb` consecutive entries.  count[digit][block]: how many entries of the block have that digit of this pass (integer
+// counts, so nothing depends on the order of the LDS atomics).  Ids outside [0, V) and the padding id are left out; *valid = entries
+// that remain.  Up to SMALL tokens are sorted by one workgroup in LDS in one launch.
+constexpr int DIGITS = 256, SORT_BLOCKS = 256, BATCH = 1024, SMALL = 2048;
 
 template <typename I>
 __device__ __forceinline__ bool entry_of(const void* ids, int64_t t, int64_t V, int64_t padding, unsigned& key) {
@@ -112,97 +107,66 @@ __device__ __forceinline__ bool entry_of(const void* ids, int64_t t, int64_t V, 
     return id >= 0 && id < V && id != padding;
 }
 
-// counts of pass 0, zeros for the later passes' counts and for the whole gradient (rows that no token names keep them)
-template <typename I>
-__global__ __launch_bounds__(256) void embed_count_kernel(const void* ids, int64_t T, int64_t V, int64_t padding, int tpb, int nblk, int passes,
-                                                          unsigned* count, void* dw, int64_t dw_bytes) {
+// zeros for the whole gradient (rows that no token names keep them): blocks [first, gridDim.x)
+__device__ __forceinline__ void clear_rows(void* dw, int64_t bytes, int first) {
+    const int64_t n16 = bytes / 16, step = (int64_t)(gridDim.x - first) * 256, i0 = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x;
+    const u32x4_t z = {0u, 0u, 0u, 0u};
+    for (int64_t i = i0; i < n16; i += step) reinterpret_cast<u32x4_t*>(dw)[i] = z;
+    if (i0 < bytes % 16) ((char*)dw)[n16 * 16 + i0] = 0;
+}
+
+// counts of one pass; the first one also clears the gradient
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(256) void embed_count_kernel(const void* ids, const uint2* in, int64_t T, int64_t V, int64_t padding, int tpb, int nblk,
+                                                          int pass, unsigned* count, const unsigned* valid, void* dw, int64_t dw_bytes) {
     __shared__ unsigned h[DIGITS];
     const int tid = threadIdx.x;
     if ((int)blockIdx.x < nblk) {
         h[tid] = 0;
         __syncthreads();
-        const int64_t t0 = (int64_t)blockIdx.x * tpb, t1 = t0 + tpb < T ? t0 + tpb : T;
+        const int64_t n = FIRST ? T : (int64_t)*valid, t0 = (int64_t)blockIdx.x * tpb, t1 = t0 + tpb < n ? t0 + tpb : n;
         for (int64_t t = t0 + tid; t < t1; t += 256) {
             unsigned key;
-            if (entry_of<I>(ids, t, V, padding, key)) atomicAdd(&h[key & 255u], 1u);
+            bool live = true;
+            if constexpr (FIRST) live = entry_of<I>(ids, t, V, padding, key);
+            else key = in[t].x;
+            if (live) atomicAdd(&h[key >> (8 * pass) & 255u], 1u);
         }
         __syncthreads();
         count[tid * nblk + blockIdx.x] = h[tid];
-        for (int p = 1; p < passes; ++p) count[(p * DIGITS + tid) * nblk + blockIdx.x] = 0;
     }
-    const int64_t n16 = dw_bytes / 16, step = (int64_t)gridDim.x * 256, i0 = (int64_t)blockIdx.x * 256 + tid;
-    const u32x4_t z = {0u, 0u, 0u, 0u};
-    for (int64_t i = i0; i < n16; i += step) reinterpret_cast<u32x4_t*>(dw)[i] = z;
-    if (i0 < dw_bytes % 16) ((char*)dw)[n16 * 16 + i0] = 0;
+    if (FIRST) clear_rows(dw, dw_bytes, 0);
 }
 
-template <typename I, bool FIRST>
-__global__ __launch_bounds__(256) void embed_scatter_kernel(const void* ids, const uint2* in, uint2* out, int64_t T, int64_t V, int64_t padding,
-                                                            int tpb, int nblk, int pass, int passes, unsigned* count, unsigned* valid) {
-    __shared__ unsigned run[DIGITS], wcount[4][DIGITS], wsum[4];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, blk = blockIdx.x;
-    // where this block's entries of digit `tid` begin: all smaller digits, and the same digit of the blocks before
-    unsigned before = 0, total = 0;
-    const unsigned* c = count + ((int64_t)pass * DIGITS + tid) * nblk;
-    for (int i = 0; i < nblk; ++i) {
-        const unsigned x = c[i];
-        before += i < blk ? x : 0;
-        total += x;
-    }
-    unsigned inc = total;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned y = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += y;
-    }
-    if (lane == 63) wsum[w] = inc;
-    __syncthreads();
-    unsigned base = inc - total;
-    for (int i = 0; i < w; ++i) base += wsum[i];
-    run[tid] = base + before;
-    if (blk == 0 && tid == 255) *valid = base + total;
-    const int64_t n = FIRST ? T : (int64_t)(wsum[0] + wsum[1] + wsum[2] + wsum[3]);
-    const int64_t t0 = (int64_t)blk * tpb, t1 = t0 + tpb < n ? t0 + tpb : n;
+// One batch of BATCH entries (a wave owns 256 consecutive ones, four of a lane): places of equal digits ascend with the entry.  run[digit]
+// = the next free place, on entry and on return.
+struct Ranker {
+    unsigned run[DIGITS], wcount[4][DIGITS];
 
-    for (int64_t b0 = t0; b0 < t1; b0 += BATCH) {                          // a wave owns 256 consecutive entries of the batch
-        unsigned key[4], idx[4];
-        bool live[4];
+    template <typename Put>
+    __device__ __forceinline__ void batch(const unsigned (&key)[4], const unsigned (&idx)[4], const bool (&live)[4], int shift, Put put) {
+        const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
         __syncthreads();                                                   // run[] is final, wcount[] free
 #pragma unroll
         for (int i = 0; i < 4; ++i) wcount[i][tid] = 0;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t t = b0 + 256 * w + 64 * i + lane;
-            live[i] = t < t1;
-            key[i] = idx[i] = 0;
-            if (live[i]) {
-                if constexpr (FIRST) {
-                    live[i] = entry_of<I>(ids, t, V, padding, key[i]);
-                    idx[i] = (unsigned)t;
-                } else {
-                    const uint2 e = in[t];
-                    key[i] = e.x; idx[i] = e.y;
-                }
-            }
-            if (live[i]) atomicAdd(&wcount[w][key[i] >> (8 * pass) & 255u], 1u);
-        }
+        for (int i = 0; i < 4; ++i)
+            if (live[i]) atomicAdd(&wcount[w][key[i] >> shift & 255u], 1u);
         __syncthreads();
-        {
-            unsigned at = run[tid];
+        unsigned at = run[tid];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned x = wcount[i][tid];
-                wcount[i][tid] = at;
-                at += x;
-            }
-            run[tid] = at;
+        for (int i = 0; i < 4; ++i) {
+            const unsigned x = wcount[i][tid];
+            wcount[i][tid] = at;
+            at += x;
         }
+        run[tid] = at;
         __syncthreads();
         volatile unsigned* const place = wcount[w];                        // this wave's next free place of every digit
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const unsigned dig = key[i] >> (8 * pass) & 255u;
+            const unsigned dig = key[i] >> shift & 255u;
             unsigned long long same = __builtin_amdgcn_ballot_w64(live[i]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -216,18 +180,140 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const void* ids, con
             __builtin_amdgcn_wave_barrier();
             if (live[i] && rank == 0) place[dig] = to + all;
             __builtin_amdgcn_wave_barrier();
-            if (live[i]) {
-                out[to] = make_uint2(key[i], idx[i]);
-                if (pass + 1 < passes)
-                    atomicAdd(&count[((int64_t)(pass + 1) * DIGITS + (key[i] >> (8 * pass + 8) & 255u)) * nblk + to / (unsigned)tpb], 1u);
-            }
+            if (live[i]) put(to, key[i], idx[i]);
         }
     }
+    // exclusive sums over the digits of `total`, one digit a thread; *all = their sum
+    __device__ __forceinline__ unsigned before(unsigned total, unsigned* all) {
+        __shared__ unsigned wsum[4];
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        unsigned inc = total;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned y = __shfl_up(inc, o, 64);
+            if (lane >= o) inc += y;
+        }
+        __syncthreads();
+        if (lane == 63) wsum[w] = inc;
+        __syncthreads();
+        unsigned base = inc - total;
+        for (int i = 0; i < w; ++i) base += wsum[i];
+        *all = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+        return base;
+    }
+};
+
+template <typename I, bool FIRST>
+__global__ __launch_bounds__(256) void embed_scatter_kernel(const void* ids, const uint2* in, uint2* out, int64_t T, int64_t V, int64_t padding,
+                                                            int tpb, int nblk, int pass, const unsigned* count, unsigned* valid) {
+    __shared__ Ranker rk;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, blk = blockIdx.x;
+    // where this block's entries of digit `tid` begin: all smaller digits, and the same digit of the blocks before
+    unsigned before = 0, total = 0;
+    const unsigned* c = count + (int64_t)tid * nblk;
+    int i = 0;
+    for (; i + 16 <= nblk; i += 16) {                                      // sixteen loads in flight
+        unsigned x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = c[i + j];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            before += i + j < blk ? x[j] : 0;
+            total += x[j];
+        }
+    }
+    for (; i < nblk; ++i) {
+        const unsigned x = c[i];
+        before += i < blk ? x : 0;
+        total += x;
+    }
+    unsigned all;
+    rk.run[tid] = rk.before(total, &all) + before;
+    if (FIRST && blk == 0 && tid == 0) *valid = all;
+    const int64_t n = FIRST ? T : (int64_t)all, t0 = (int64_t)blk * tpb, t1 = t0 + tpb < n ? t0 + tpb : n;
+    for (int64_t b0 = t0; b0 < t1; b0 += BATCH) {
+        unsigned key[4], idx[4];
+        bool live[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t t = b0 + 256 * w + 64 * k + lane;
+            live[k] = t < t1;
+            key[k] = idx[k] = 0;
+            if (live[k]) {
+                if constexpr (FIRST) {
+                    live[k] = entry_of<I>(ids, t, V, padding, key[k]);
+                    idx[k] = (unsigned)t;
+                } else {
+                    const uint2 e = in[t];
+                    key[k] = e.x;
+                    idx[k] = e.y;
+                }
+            }
+        }
+        rk.batch(key, idx, live, 8 * pass, [&](unsigned to, unsigned k, unsigned t) { out[to] = make_uint2(k, t); });
+    }
+}
+
+// All passes of up to SMALL tokens in one workgroup; the others clear the gradient.
+template <typename I>
+__global__ __launch_bounds__(256) void embed_sort_small_kernel(const void* ids, uint2* out, int T, int64_t V, int64_t padding, int passes,
+                                                               unsigned* valid, void* dw, int64_t dw_bytes) {
+    __shared__ Ranker rk;
+    __shared__ uint2 buf[2][SMALL];
+    __shared__ unsigned h[DIGITS];
+    if (blockIdx.x) {
+        clear_rows(dw, dw_bytes, 1);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int n = T;
+    for (int pass = 0; pass < passes; ++pass) {
+        h[tid] = 0;
+        __syncthreads();
+        const auto entry = [&](int t, unsigned& key, unsigned& idx) {
+            bool live = t < n;
+            key = idx = 0;
+            if (live) {
+                if (pass == 0) {
+                    live = entry_of<I>(ids, t, V, padding, key);
+                    idx = (unsigned)t;
+                } else {
+                    const uint2 e = buf[(pass + 1) & 1][t];
+                    key = e.x;
+                    idx = e.y;
+                }
+            }
+            return live;
+        };
+        for (int t = tid; t < n; t += 256) {
+            unsigned key, idx;
+            if (entry(t, key, idx)) atomicAdd(&h[key >> (8 * pass) & 255u], 1u);
+        }
+        __syncthreads();
+        unsigned all;
+        rk.run[tid] = rk.before(h[tid], &all);
+        const bool last = pass + 1 == passes;
+        for (int b0 = 0; b0 < n; b0 += BATCH) {
+            unsigned key[4], idx[4];
+            bool live[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) live[k] = entry(b0 + 256 * w + 64 * k + lane, key[k], idx[k]);
+            rk.batch(key, idx, live, 8 * pass, [&](unsigned to, unsigned k, unsigned t) {
+                if (last) out[to] = make_uint2(k, t);
+                else buf[pass & 1][to] = make_uint2(k, t);
+            });
+        }
+        n = (int)all;
+        __syncthreads();
+    }
+    if (tid == 0) *valid = (unsigned)n;
 }
 
 // ---- sums of runs of equal ids --------------------------------------------------------------------------------------------------------
 // A wave takes `chunk` sorted positions and 64 pieces of columns.  A run inside the chunk goes straight to dW; the part of a run that
 // continues from the chunk before goes to part[c][0], the part of one that starts here and goes on to part[c][1].
+constexpr int GROUP = 32;        // positions whose ids and tokens one load brings: lane i holds position i
+
 template <int TY, bool VEC>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint2* sorted, const unsigned* valid, const void* dout, void* dw, float* part,
                                                         int C, int chunk, int nseg, float scale) {
@@ -238,92 +324,135 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint2* sorted, con
     const int col = ((int)(u - c * nseg) * 64 + lane) * P::N;
     if (p0 >= p1) return;
     const bool in = col < C;
-    bool head = p0 > 0 && sorted[p0 - 1].x == sorted[p0].x;                // the first run came from the chunk before
+    unsigned prev = p0 > 0 ? sorted[p0 - 1].x : 0xffffffffu;               // 0xffffffff: no id, they are below 2^31
+    bool first = true, head = false;
     float acc[P::N];
 #pragma unroll
     for (int i = 0; i < P::N; ++i) acc[i] = 0.f;
     constexpr int AHEAD = 8;
-    for (int64_t q = p0; q < p1; q += AHEAD) {
-        uint2 e[AHEAD + 1];
-        P x[AHEAD];
+    for (int64_t q0 = p0; q0 < p1; q0 += GROUP) {
+        uint2 e = make_uint2(0xffffffffu, 0u);
+        if (lane <= GROUP && q0 + lane < n) e = sorted[q0 + lane];
+        if (first) head = prev == (unsigned)__builtin_amdgcn_readlane((int)e.x, 0);      // the first run came from the chunk before
+        first = false;
+        const int m = p1 - q0 < GROUP ? (int)(p1 - q0) : GROUP;
+        for (int j0 = 0; j0 < m; j0 += AHEAD) {
+            P x[AHEAD];
 #pragma unroll
-        for (int i = 0; i <= AHEAD; ++i) {
-            e[i] = make_uint2(0xffffffffu, 0u);                            // no id: ids are below 2^31
-            if (q + i < n) e[i] = sorted[q + i];
-        }
+            for (int i = 0; i < AHEAD; ++i)                                // no branch: all in flight (behind the end: the last row again)
+                x[i].load(dout, (int64_t)(unsigned)__builtin_amdgcn_readlane((int)e.y, j0 + i < m ? j0 + i : m - 1) * C + (in ? col : 0));
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            if (q + i < p1 && in) x[i].load(dout, (int64_t)e[i].y * C + col);
+            for (int i = 0; i < AHEAD; ++i) {
+                if (j0 + i >= m) break;
+                if (in) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (q + i >= p1) break;
-            if (in) {
-#pragma unroll
-                for (int j = 0; j < P::N; ++j) acc[j] += x[i].x[j];
-            }
-            const bool ends = e[i].x != e[i + 1].x, last = q + i + 1 == p1;
-            if (!ends && !last) continue;
-            if (in) {
-                if (ends && !head) {
-                    P r;
-#pragma unroll
-                    for (int j = 0; j < P::N; ++j) r.x[j] = acc[j] * scale;
-                    r.store(dw, (int64_t)e[i].x * C + col);
-                } else {
-                    float* to = part + (2 * c + (head ? 0 : 1)) * C + col;
-#pragma unroll
-                    for (int j = 0; j < P::N; ++j) to[j] = acc[j];
+                    for (int j = 0; j < P::N; ++j) acc[j] += x[i].x[j];
                 }
-            }
+                const unsigned id = (unsigned)__builtin_amdgcn_readlane((int)e.x, j0 + i);
+                const bool ends = id != (unsigned)__builtin_amdgcn_readlane((int)e.x, j0 + i + 1), last = q0 + j0 + i + 1 == p1;
+                if (!ends && !last) continue;
+                if (in) {
+                    if (ends && !head) {
+                        P r;
 #pragma unroll
-            for (int j = 0; j < P::N; ++j) acc[j] = 0.f;
-            head = false;
+                        for (int j = 0; j < P::N; ++j) r.x[j] = acc[j] * scale;
+                        r.store(dw, (int64_t)id * C + col);
+                    } else {
+                        float* to = part + (2 * c + (head ? 0 : 1)) * C + col;
+#pragma unroll
+                        for (int j = 0; j < P::N; ++j) to[j] = acc[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < P::N; ++j) acc[j] = 0.f;
+                head = false;
+            }
         }
     }
 }
 
-// A run that starts in chunk c and goes on: its part there and those of the chunks that follow, in order
+// A run that starts in chunk c and goes on: its part there, then those of the chunks that follow.  A wave takes one run and 64 pieces of
+// columns; a run of more than LONG parts is summed by the four waves of its workgroup, a contiguous quarter each, added in order.
+constexpr int LONG = 16;
+
 template <int TY, bool VEC>
-__global__ __launch_bounds__(256) void embed_join_kernel(const uint2* sorted, const unsigned* valid, void* dw, const float* part, int C,
-                                                         int chunk, int nseg, float scale) {
+__global__ __launch_bounds__(256) void embed_join_kernel(const uint2* sorted, const unsigned* valid, void* dw, const float* part, int64_t T, int C,
+                                                         int chunk, int64_t chunks, int nseg, float scale) {
     using P = Piece<TY, VEC>;
-    const int lane = threadIdx.x & 63;
-    const int64_t n = *valid, u = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t c = u / nseg, p0 = c * chunk, p1 = p0 + chunk;
-    const int col = ((int)(u - c * nseg) * 64 + lane) * P::N;
-    if (p1 >= n) return;                                                   // the last chunk's runs end in it
-    const unsigned id = sorted[p1 - 1].x;
-    if (sorted[p1].x != id) return;
-    if (sorted[p0].x == id && p0 > 0 && sorted[p0 - 1].x == id) return;    // it started before this chunk
-    int64_t end = c + 1;                                                   // last chunk that holds a part of the run
-    {
-        int64_t lo = c + 1, hi = (n - 1) / chunk;                          // first position of chunk lo has the id
-        while (lo < hi) {
-            const int64_t mid = (lo + hi + 1) / 2;
-            if (sorted[mid * chunk].x == id) lo = mid;
-            else hi = mid - 1;
+    __shared__ float sums[4][64 * P::N];
+    __shared__ int64_t run_end[4];
+    __shared__ unsigned run_id[4];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t u0 = (int64_t)blockIdx.x * 4, u = u0 + w, c = u / nseg, p0 = c * chunk, p1 = p0 + chunk;
+    // one load for the ids around this chunk's borders and one for the first ids of the next 64 chunks (entries behind *valid hold anything)
+    const int64_t near = lane == 0 ? p1 - 1 : lane == 1 ? p1 : lane == 2 ? p0 : p0 - 1, next = (c + 1 + lane) * chunk;
+    const unsigned e = c < chunks && near >= 0 && near < T ? sorted[near].x : 0u, f = next < T ? sorted[next].x : 0u;
+    const int64_t n = *valid, most = (n - 1) / chunk;
+    const unsigned id = (unsigned)__builtin_amdgcn_readlane((int)e, 0);
+    const bool goes_on = c < chunks && p1 < n && (unsigned)__builtin_amdgcn_readlane((int)e, 1) == id;
+    const bool came = (unsigned)__builtin_amdgcn_readlane((int)e, 2) == id && p0 > 0 && (unsigned)__builtin_amdgcn_readlane((int)e, 3) == id;
+    int64_t end = -1;                                                      // last chunk that holds a part of the run that starts here
+    if (goes_on && !came) {
+        end = c + __builtin_ctzll(~__builtin_amdgcn_ballot_w64(c + 1 + lane <= most && f == id) | 1ull << 63);
+        while (end == c + 63 || (end > c + 63 && (end - c) % 64 == 63)) {  // all of them: look further
+            const int64_t k = end + 1 + lane;
+            const unsigned long long has = __builtin_amdgcn_ballot_w64(k <= most && sorted[(k <= most ? k : most) * chunk].x == id);
+            const int run = has == ~0ull ? 64 : __builtin_ctzll(~has);
+            end += run;
+            if (run < 64) break;
         }
-        end = lo;
     }
-    if (col >= C) return;
-    P acc;
+    const int seg = (int)(u - c * nseg);
+    const auto total = [&](int64_t cc, int64_t k0, int64_t k1, bool with_start, int col, float (&acc)[P::N]) {
+        const float* const at = part + (col < C ? col : 0);
 #pragma unroll
-    for (int j = 0; j < P::N; ++j) acc.x[j] = part[(2 * c + 1) * C + col + j];
-    constexpr int AHEAD = 8;
-    for (int64_t k = c + 1; k <= end; k += AHEAD) {
-        float x[AHEAD][P::N];
+        for (int j = 0; j < P::N; ++j) acc[j] = with_start ? at[(2 * cc + 1) * C + j] : 0.f;
+        constexpr int AHEAD = 8;
+        for (int64_t k = k0; k <= k1; k += AHEAD) {
+            float x[AHEAD][P::N];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
+            for (int i = 0; i < AHEAD; ++i)                                // no branch: all in flight
 #pragma unroll
-            for (int j = 0; j < P::N; ++j) x[i][j] = k + i <= end ? part[2 * (k + i) * C + col + j] : 0.f;
+                for (int j = 0; j < P::N; ++j) x[i][j] = at[2 * (k + i <= k1 ? k + i : k1) * C + j];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
+            for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-            for (int j = 0; j < P::N; ++j) acc.x[j] += x[i][j];
+                for (int j = 0; j < P::N; ++j) acc[j] += k + i <= k1 ? x[i][j] : 0.f;
+        }
+    };
+    const bool is_long = end - c > LONG && end >= 0;
+    if (lane == 0) {
+        run_end[w] = is_long ? end : -1;
+        run_id[w] = id;
     }
+    if (end >= 0 && !is_long) {
+        const int col = (seg * 64 + lane) * P::N;
+        P r;
+        total(c, c + 1, end, true, col, r.x);
+        if (col < C) {
 #pragma unroll
-    for (int j = 0; j < P::N; ++j) acc.x[j] *= scale;
-    acc.store(dw, (int64_t)id * C + col);
+            for (int j = 0; j < P::N; ++j) r.x[j] *= scale;
+            r.store(dw, (int64_t)id * C + col);
+        }
+    }
+    __syncthreads();
+    for (int i = 0; i < 4; ++i) {
+        const int64_t last = run_end[i];
+        if (last < 0) continue;                                            // the same for all four waves
+        const int64_t uu = u0 + i, cc = uu / nseg, each = (last - cc + 3) / 4, k0 = cc + 1 + w * each, k1 = k0 + each - 1 < last ? k0 + each - 1 : last;
+        const int col = ((int)(uu - cc * nseg) * 64 + lane) * P::N;
+        P r;
+        total(cc, k0, k1, w == 0, col, r.x);
+#pragma unroll
+        for (int j = 0; j < P::N; ++j) sums[w][64 * j + lane] = r.x[j];
+        __syncthreads();
+        if (w == 0 && col < C) {
+#pragma unroll
+            for (int j = 0; j < P::N; ++j) r.x[j] = (((r.x[j] + sums[1][64 * j + lane]) + sums[2][64 * j + lane]) + sums[3][64 * j + lane]) * scale;
+            r.store(dw, (int64_t)run_id[i] * C + col);
+        }
+        __syncthreads();
+    }
 }
 
 struct Plan {
@@ -346,7 +475,7 @@ Plan plan(int64_t T, int64_t V, int C) {
     p.chunks = (T + p.chunk - 1) / p.chunk;
     p.pairs = up16((size_t)T * 8);
     p.counts = 2 * p.pairs;
-    p.parts = p.counts + up16(((size_t)p.passes * DIGITS * p.nblk + 4) * 4);
+    p.parts = p.counts + up16(((size_t)DIGITS * p.nblk + 4) * 4);
     p.total = p.parts + (size_t)p.chunks * 2 * C * 4;
     return p;
 }
@@ -369,14 +498,15 @@ int go_fwd(const void* ids, int i64, const void* w, int64_t ws, int64_t V, void*
 }
 
 template <int TY, bool VEC>
-int go_sums(const uint2* sorted, const unsigned* valid, const void* dout, void* dw, float* part, int C, const Plan& p, float scale, hipStream_t s) {
+int go_sums(const uint2* sorted, const unsigned* valid, const void* dout, void* dw, float* part, int64_t T, int C, const Plan& p, float scale, hipStream_t s) {
     const int per = 64 * Piece<TY, VEC>::N, nseg = (C + per - 1) / per;
     const int64_t blocks = (p.chunks * nseg + 3) / 4;
     if (blocks > 0x7fffffff) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);
     FAVAE_KLAUNCH((embed_sum_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dout, dw, part, C, p.chunk, nseg, scale);
     FAVAE_CHECK_LAUNCH();
     if (p.chunks > 1) {
-        FAVAE_KLAUNCH((embed_join_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dw, (const float*)part, C, p.chunk, nseg, scale);
+        FAVAE_KLAUNCH((embed_join_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dw, (const float*)part, T, C, p.chunk,
+                      p.chunks, nseg, scale);
         FAVAE_CHECK_LAUNCH();
     }
     return FAVAE_OK;
@@ -416,27 +546,42 @@ extern "C" int favae_embed_bwd(const void* ids, int ids_are_64bit, const void* d
     const hipStream_t s = (hipStream_t)stream;
     uint2* const buf[2] = {(uint2*)ws, (uint2*)((char*)ws + p.pairs)};
     unsigned* const count = (unsigned*)((char*)ws + p.counts);
-    unsigned* const valid = count + (size_t)p.passes * DIGITS * p.nblk;
+    unsigned* const valid = count + (size_t)DIGITS * p.nblk;
     float* const part = (float*)((char*)ws + p.parts);
     const int64_t dw_bytes = V * C * (dtype == F32 ? 4 : 2);
-    const int64_t zb = (dw_bytes + 65535) / 65536;
-    const int grid = (int)(zb > 2048 ? 2048 : zb > p.nblk ? zb : p.nblk);
-    if (ids_are_64bit) FAVAE_KLAUNCH((embed_count_kernel<int64_t>), dim3(grid), dim3(256), 0, s, ids, T, V, padding_idx, p.tpb, p.nblk, p.passes, count, dweight, dw_bytes);
-    else FAVAE_KLAUNCH((embed_count_kernel<int32_t>), dim3(grid), dim3(256), 0, s, ids, T, V, padding_idx, p.tpb, p.nblk, p.passes, count, dweight, dw_bytes);
-    FAVAE_CHECK_LAUNCH();
-    for (int k = 0; k < p.passes; ++k) {
-        const uint2* in = buf[(k + 1) & 1];
-        uint2* out = buf[k & 1];
-        if (k) FAVAE_KLAUNCH((embed_scatter_kernel<int32_t, false>), dim3(p.nblk), dim3(256), 0, s, ids, in, out, T, V, padding_idx, p.tpb, p.nblk, k, p.passes, count, valid);
-        else if (ids_are_64bit) FAVAE_KLAUNCH((embed_scatter_kernel<int64_t, true>), dim3(p.nblk), dim3(256), 0, s, ids, in, out, T, V, padding_idx, p.tpb, p.nblk, k, p.passes, count, valid);
-        else FAVAE_KLAUNCH((embed_scatter_kernel<int32_t, true>), dim3(p.nblk), dim3(256), 0, s, ids, in, out, T, V, padding_idx, p.tpb, p.nblk, k, p.passes, count, valid);
+    const int64_t zb = (dw_bytes + 65535) / 65536;                         // workgroups that clear the gradient
+    const int zeros = (int)(zb > 2048 ? 2048 : zb);
+    const uint2* sorted = buf[0];
+    if (T <= SMALL) {
+        if (ids_are_64bit) FAVAE_KLAUNCH((embed_sort_small_kernel<int64_t>), dim3(1 + zeros), dim3(256), 0, s, ids, buf[0], (int)T, V, padding_idx, p.passes, valid, dweight, dw_bytes);
+        else FAVAE_KLAUNCH((embed_sort_small_kernel<int32_t>), dim3(1 + zeros), dim3(256), 0, s, ids, buf[0], (int)T, V, padding_idx, p.passes, valid, dweight, dw_bytes);
         FAVAE_CHECK_LAUNCH();
+    } else {
+        const dim3 g0(zeros > p.nblk ? zeros : p.nblk), g(p.nblk), t(256);
+        for (int k = 0; k < p.passes; ++k) {
+            const uint2* in = buf[(k + 1) & 1];
+            uint2* out = buf[k & 1];
+            if (k) {
+                FAVAE_KLAUNCH((embed_count_kernel<int32_t, false>), g, t, 0, s, ids, in, T, V, padding_idx, p.tpb, p.nblk, k, count, valid, dweight, dw_bytes);
+                FAVAE_CHECK_LAUNCH();
+                FAVAE_KLAUNCH((embed_scatter_kernel<int32_t, false>), g, t, 0, s, ids, in, out, T, V, padding_idx, p.tpb, p.nblk, k, count, valid);
+            } else if (ids_are_64bit) {
+                FAVAE_KLAUNCH((embed_count_kernel<int64_t, true>), g0, t, 0, s, ids, in, T, V, padding_idx, p.tpb, p.nblk, k, count, valid, dweight, dw_bytes);
+                FAVAE_CHECK_LAUNCH();
+                FAVAE_KLAUNCH((embed_scatter_kernel<int64_t, true>), g, t, 0, s, ids, in, out, T, V, padding_idx, p.tpb, p.nblk, k, count, valid);
+            } else {
+                FAVAE_KLAUNCH((embed_count_kernel<int32_t, true>), g0, t, 0, s, ids, in, T, V, padding_idx, p.tpb, p.nblk, k, count, valid, dweight, dw_bytes);
+                FAVAE_CHECK_LAUNCH();
+                FAVAE_KLAUNCH((embed_scatter_kernel<int32_t, true>), g, t, 0, s, ids, in, out, T, V, padding_idx, p.tpb, p.nblk, k, count, valid);
+            }
+            FAVAE_CHECK_LAUNCH();
+            sorted = out;
+        }
     }
-    const uint2* sorted = buf[(p.passes - 1) & 1];
     const bool vec = vec_ok(dtype, C, 0, dout, dweight);
 #define GO(TY)                                                                                      \
-    return vec ? go_sums<TY, true>(sorted, valid, dout, dweight, part, C, p, scale, s)              \
-               : go_sums<TY, false>(sorted, valid, dout, dweight, part, C, p, scale, s)
+    return vec ? go_sums<TY, true>(sorted, valid, dout, dweight, part, T, C, p, scale, s)              \
+               : go_sums<TY, false>(sorted, valid, dout, dweight, part, T, C, p, scale, s)
     if (dtype == F32) GO(F32);
     if (dtype == BF16) GO(BF16);
     GO(F16);

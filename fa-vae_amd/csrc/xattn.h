@@ -346,7 +346,7 @@ template <int TY, int DP, bool KEYW> struct FwdCfg {
     static constexpr int NT = 256;
     static constexpr int NW = KEYW && TY == F32 && DP > 64 ? 2 : 4;        // waves that compute: the planes of 128 keys of 96, 128 fp32 columns
     static constexpr int ROWS = KEYW ? 32 : 32 * NW;                       // do not fit LDS, there two waves only load
-    static constexpr int WAVES = TY == F32 && DP > 64 ? 1 : 2;            // a SIMD; also keeps accumulators out of the second register file
+    static constexpr int WAVES = (TY == F32 && DP > 64) || (KEYW && DP == 128) ? 1 : 2;   // a SIMD; also keeps accumulators out of the second register file
     static constexpr int BK = KEYW ? 32 * NW : TY == F32 ? 32 : 64;
     static constexpr int KS = KEYW ? 1 : BK / 32;
     static constexpr int TILE = tile_len<TY, DP, BK>();
@@ -365,14 +365,19 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
     float* const stat = bias + C::BUFS * C::BK;                           // [2][NW][32] maxima, sums (KEYW)
     int* const red = reinterpret_cast<int*>(stat + 64 * C::NW);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int tile = id % a.tiles; id /= a.tiles;
-    const int split = id % a.nsplit, bh = id / a.nsplit;
+    // workgroups of one head follow one another on an XCD: its keys stay in that L2.  Few rows share nothing (each split reads its own
+    // keys), there the heads of a ragged batch alternate instead.
+    int id = KEYW ? blockIdx.x : xcd_remap(blockIdx.x, gridDim.x);
+    const int heads = a.B * a.Hkv;
+    const int bh = KEYW ? id % heads : id / (a.tiles * a.nsplit);
+    id = KEYW ? id / heads : id % (a.tiles * a.nsplit);
+    const int tile = id % a.tiles, split = id / a.tiles;
     const int b = bh / a.Hkv, kv = bh % a.Hkv;
     const char* const kp = (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES;
     const char* const vp = (const char*)a.v + (b * a.v_b + kv * a.v_h) * T::ES;
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
-    const int k0 = split * a.span, kend = last_key<C::NT>(pad, k0, min(a.Lk, k0 + a.span), tid, red);
+    const int k0 = split * a.span;
+    int kend = min(a.Lk, k0 + a.span);
 
     Stage<TY, DP, C::BK, C::NT> sk, sv;
     unsigned char pb[(C::BK + 63) / 64];
@@ -385,11 +390,11 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
             pb[i] = 64 * i + lane < C::BK && j < kend ? (pad ? pad[j] : 0) : 1;
         }
     };
-    if (k0 < kend) fetch(k0);
-
+    fetch(k0);                                                             // k0 < Lk; on its way while the mask is looked through
     const int row = tile * C::ROWS + (KEYW ? 0 : 32 * w) + (lane & 31);
     Frag<T::PL> qf[DP / 16];
     load_row<TY, DP>(row < a.R ? (const char*)a.q + row_at(a, bh, row, a.q_b, a.q_l, a.q_h) * T::ES : nullptr, a.D, lane, qf);
+    kend = last_key<C::NT>(pad, k0, kend, tid, red);
     f32x16 o[DP / 32];
     float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -535,6 +540,229 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
 }
 
 // -------------------------------------------------------------------------------------------------------------------------------------
+// Forward of up to 16 rows a head group (a decoding step): bound by the bytes of K and V.  16x16x32 MFMAs hold the 16 rows in half the
+// registers of the 32-row form, so that two workgroups of 128 keys a tile share a CU and one's loads run under the other's arithmetic.
+// Each wave takes 32 keys of the tile: lane l holds row l % 16 and keys 4 (l / 16) + i and 16 + 4 (l / 16) + i, which are also the
+// contraction slots of the second product.
+// -------------------------------------------------------------------------------------------------------------------------------------
+template <int TY> __device__ __forceinline__ fx4 mma16_1(s16x8 a, s16x8 b, fx4 c) {
+    if constexpr (TY == F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+}
+template <int TY>
+__device__ __forceinline__ fx4 mma16(const Frag<Ty<TY>::PL>& a, const Frag<Ty<TY>::PL>& b, fx4 c) {
+    if constexpr (TY == F32) {
+        c = mma16_1<TY>(a.p[2], b.p[0], c);
+        c = mma16_1<TY>(a.p[0], b.p[2], c);
+        c = mma16_1<TY>(a.p[1], b.p[1], c);
+        c = mma16_1<TY>(a.p[1], b.p[0], c);
+        c = mma16_1<TY>(a.p[0], b.p[1], c);
+        c = mma16_1<TY>(a.p[0], b.p[0], c);
+        return c;
+    } else {
+        return mma16_1<TY>(a.p[0], b.p[0], c);
+    }
+}
+// rows row0 + l % 16, columns 32 s + 8 (l / 16) + 0..7
+template <int TY, int DP, int ROWS>
+__device__ __forceinline__ Frag<Ty<TY>::PL> row_frag16(const short* t, int row0, int s, int lane) {
+    Frag<Ty<TY>::PL> f;
+    const int r = lane & 15;
+    const short* p = t + r * DP + 8 * ((4 * s + (lane >> 4)) ^ swizzle<DP>(r)) + row0 * DP;
+#pragma unroll
+    for (int i = 0; i < Ty<TY>::PL; ++i) f.p[i] = *reinterpret_cast<const s16x8*>(p + i * ROWS * DP);
+    return f;
+}
+// column col0 + l % 16, slots j = rows row0 + 16 (j / 4) + 4 (l / 16) + j % 4
+template <int TY, int DP, int ROWS>
+__device__ __forceinline__ Frag<Ty<TY>::PL> col_frag16(short* t, int row0, int col0, int lane) {
+    typedef __attribute__((address_space(3))) s16x4* lds4;
+    Frag<Ty<TY>::PL> f;
+    const int r = 4 * (lane >> 4) + ((lane & 15) >> 2), c = col0 / 8 + ((lane & 3) >> 1);
+    short* p = t + r * DP + 8 * (c ^ swizzle<DP>(r)) + 4 * (lane & 1) + row0 * DP;
+#pragma unroll
+    for (int i = 0; i < Ty<TY>::PL; ++i) {
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + i * ROWS * DP));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + i * ROWS * DP + 16 * DP));
+        f.p[i] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    return f;
+}
+
+template <int TY, int DP> struct TokCfg {
+    static constexpr int NT = 256;
+    static constexpr int NW = TY == F32 && DP > 64 ? 2 : 4;                // as in FwdCfg
+    static constexpr int BK = 32 * NW;
+    static constexpr int TILE = tile_len<TY, DP, BK>();
+    static constexpr int RED = NW * DP * 16 * 2;
+    static constexpr int LEN = 2 * TILE > RED ? 2 * TILE : RED;
+    static constexpr size_t LDS = LEN * 2 + BK * 4 + 32 * 4 * NW + 16;
+};
+
+template <int TY, int DP>
+__global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
+    using C = TokCfg<TY, DP>;
+    using T = Ty<TY>;
+    extern __shared__ __attribute__((aligned(16))) short lds[];
+    short* const kt = lds;
+    short* const vt = lds + C::TILE;
+    float* const bias = reinterpret_cast<float*>(lds + C::LEN);           // [BK]
+    float* const stat = bias + C::BK;                                     // [2][NW][16] maxima, sums
+    int* const red = reinterpret_cast<int*>(stat + 32 * C::NW);
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
+    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, split = blockIdx.x / heads;   // heads alternate: a ragged batch is spread evenly
+    const int b = bh / a.Hkv, kv = bh % a.Hkv;
+    const char* const kp = (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES;
+    const char* const vp = (const char*)a.v + (b * a.v_b + kv * a.v_h) * T::ES;
+    const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
+    const int k0 = split * a.span;
+    int kend = min(a.Lk, k0 + a.span);
+
+    Stage<TY, DP, C::BK, C::NT> sk, sv;
+    unsigned char pb[(C::BK + 63) / 64];
+    const auto fetch = [&](int key) {
+        sk.load(tid, a.D, kp + key * a.k_l * T::ES, a.k_l * T::ES, kend - key);
+        sv.load(tid, a.D, vp + key * a.v_l * T::ES, a.v_l * T::ES, kend - key);
+#pragma unroll
+        for (int i = 0; i < (C::BK + 63) / 64; ++i) {
+            const int j = key + 64 * i + lane;
+            pb[i] = j < kend ? (pad ? pad[j] : 0) : 1;
+        }
+    };
+    fetch(k0);                                                             // k0 < Lk
+    const int row = lane & 15;
+    Frag<T::PL> qf[DP / 32];
+    {
+        const char* const q = row < a.R ? (const char*)a.q + row_at(a, bh, row, a.q_b, a.q_l, a.q_h) * T::ES : nullptr;
+#pragma unroll
+        for (int s = 0; s < DP / 32; ++s) {
+            const int col = 32 * s + 8 * quad;
+            ux4 x[T::ES / 2] = {};
+            if (q && col < a.D) {
+#pragma unroll
+                for (int i = 0; i < T::ES / 2; ++i) x[i] = reinterpret_cast<const ux4*>(q + col * T::ES)[i];
+            }
+            if constexpr (TY == F32) {
+                float f[8];
+                const fx4 lo = __builtin_bit_cast(fx4, x[0]), hi = __builtin_bit_cast(fx4, x[1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { f[j] = lo[j]; f[4 + j] = hi[j]; }
+                qf[s] = make_frag<TY>(f);
+            } else {
+                qf[s].p[0] = __builtin_bit_cast(s16x8, x[0]);
+            }
+        }
+    }
+    kend = last_key<C::NT>(pad, k0, kend, tid, red);
+    fx4 o[DP / 16];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) o[t] = (fx4){0.f, 0.f, 0.f, 0.f};
+
+    for (int key = k0; key < kend; key += C::BK) {
+        unsigned long long word[(C::BK + 63) / 64];
+        bool all = true;
+#pragma unroll
+        for (int i = 0; i < (C::BK + 63) / 64; ++i) {
+            word[i] = __builtin_amdgcn_ballot_w64(pb[i] == 0);
+            all = all && word[i] == ~0ull;
+        }
+        __syncthreads();
+        if (!all) {
+            const auto keep = [&](int r) { return (bool)((r >= 64 ? word[(C::BK + 63) / 64 - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
+            sk.blank(tid, keep);
+            sv.blank(tid, keep);
+            if (tid < C::BK) bias[tid] = keep(tid) ? 0.f : -INFINITY;
+        }
+        sk.store(kt, tid);
+        sv.store(vt, tid);
+        __syncthreads();
+        if (key + C::BK < kend) fetch(key + C::BK);
+        if (w >= C::NW) continue;
+
+        fx4 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = (fx4){0.f, 0.f, 0.f, 0.f};
+            if (!all) s[t] = *reinterpret_cast<const fx4*>(bias + 32 * w + 16 * t + 4 * quad);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) s[t] = mma16<TY>(row_frag16<TY, DP, C::BK>(kt, 32 * w + 16 * t, d, lane), qf[d], s[t]);
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > LAZY)) {
+            const float to = fmaxf(m, mx), f = to > m ? exp2_f((m - to) * a.c) : 1.f;
+            l *= f;
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) o[t] *= f;
+            m = to;
+        }
+        const float sh = T::FSHIFT - (m == -INFINITY ? 0.f : m * a.c);
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i] = exp2_f(fmaf(s[i >> 2][i & 3], a.c, sh));
+            l += p[i];
+        }
+        const Frag<T::PL> pf = make_frag<TY>(p);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) o[t] = mma16<TY>(col_frag16<TY, DP, C::BK>(vt, 32 * w, 16 * t, lane), pf, o[t]);
+    }
+
+    float lt = l + __shfl_xor(l, 16, 64);
+    lt += __shfl_xor(lt, 32, 64);
+    if (quad == 0 && w < C::NW) {
+        stat[w * 16 + row] = m;
+        stat[(C::NW + w) * 16 + row] = lt;
+    }
+    __syncthreads();                                                        // also: every wave is done with the tiles
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < C::NW; ++i) M = fmaxf(M, stat[i * 16 + row]);
+    const float mr = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int i = 0; i < C::NW; ++i) {
+        const float x = stat[i * 16 + row];
+        L += x == -INFINITY ? 0.f : exp2_f((x - mr) * a.c) * stat[(C::NW + i) * 16 + row];
+    }
+    const float f = m == -INFINITY ? 0.f : exp2_f((m - mr) * a.c);
+    const float inv = L == 0.f ? 0.f : f / L;
+    float* acc = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (w < C::NW) acc[(w * DP + 16 * t + 4 * quad + i) * 16 + row] = o[t][i] * inv;
+    __syncthreads();
+    if (w == 0 && quad == 0 && row < a.R) {
+        const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L) - T::FSHIFT);
+        if (a.nsplit > 1) a.part_lse[((int64_t)split * heads + bh) * a.R + row] = ls;
+        else if (a.lse) a.lse[(int64_t)bh * a.R + row] = L == 0.f ? INFINITY : ls;
+    }
+    const int nq = a.D / 4;
+    for (int e = tid; e < a.R * nq; e += C::NT) {
+        const int r = e / nq, d = 4 * (e % nq);
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < C::NW; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] += acc[(i * DP + d + j) * 16 + r];
+        if (a.nsplit > 1) {
+            put4<F32>(a.part, (((int64_t)split * heads + bh) * a.R + r) * a.D + d, x[0], x[1], x[2], x[3]);
+        } else {
+            const int64_t at = out_at(a, bh, r) + d;
+            put4<TY>(a.o, at, x[0], x[1], x[2], x[3]);
+            if (a.o32) put4<F32>(a.o32, at, x[0], x[1], x[2], x[3]);
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------------------------------------
 // fp16 gradients of scores: p (dp - delta) has the range of dout times v, which 5 exponent bits need not hold.  Each lane keeps a power
 // of two for its accumulator column: the largest value seen is brought to 2^10 and the accumulators are rescaled when a later tile
 // exceeds 2^14.  It starts at 2^120, so that the first value sets it.  (bf16 and the three-plane form have fp32's exponents: factor 1.)
@@ -569,7 +797,7 @@ template <int TY, int NACC> struct DsScale {
 // transposed as in the forward pass (K and V rows are A operands), dq^T accumulates K^T ds^T.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DqCfg {
-    static constexpr int BK = TY == F32 ? 32 : 64, NT = 256, ROWS = 128;
+    static constexpr int BK = TY == F32 || DP == 128 ? 32 : 64, NT = 256, ROWS = 128;
     static constexpr int WAVES = TY == F32 && DP > 64 ? 1 : 2;
     static constexpr int TILE = tile_len<TY, DP, BK>();
     static constexpr int BUFS = bufs_of(TILE, WAVES);
@@ -591,7 +819,8 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
     const char* const kp = (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES;
     const char* const vp = (const char*)a.v + (b * a.v_b + kv * a.v_h) * T::ES;
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
-    const int k0 = split * a.span, kend = last_key<C::NT>(pad, k0, min(a.Lk, k0 + a.span), tid, red);
+    const int k0 = split * a.span;
+    int kend = min(a.Lk, k0 + a.span);
 
     Stage<TY, DP, C::BK, C::NT> sk, sv;
     unsigned char pb;
@@ -601,7 +830,8 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
         const int j = key + lane;
         pb = lane < C::BK && j < kend ? (pad ? pad[j] : 0) : 1;
     };
-    if (k0 < kend) fetch(k0);
+    fetch(k0);                                                             // k0 < Lk; on its way while the mask is looked through
+    kend = last_key<C::NT>(pad, k0, kend, tid, red);
 
     const int row = tile * C::ROWS + 32 * w + (lane & 31);
     const bool in = row < a.R;
@@ -815,9 +1045,45 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
 }
 
 // ---- joining splits -------------------------------------------------------------------------------------------------------------------
-// forward: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  A workgroup owns a row: its threads take four columns of every
-// (256 / columns)-th split, so that one latency covers many splits, and are summed in a fixed order.
-constexpr int MOST_SPLITS = 1024;
+// forward: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  Few splits: a thread owns four columns of a row.
+constexpr int MOST_SPLITS = 1024, FEW_SPLITS = 8;
+
+template <int TY>
+__global__ __launch_bounds__(256) void join_few_kernel(const Args a) {
+    const int nq = a.D / 4;
+    const int64_t rows = (int64_t)a.B * a.Hkv * a.R, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= rows * nq) return;
+    const int64_t fr = e / nq;
+    const int d = 4 * (int)(e % nq);
+    float ls[FEW_SPLITS], M = -INFINITY, W = 0.f;
+    fx4 y[FEW_SPLITS], x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < FEW_SPLITS; ++s) {
+        ls[s] = -INFINITY;
+        y[s] = x;
+        if (s < a.nsplit) {
+            ls[s] = a.part_lse[s * rows + fr];
+            y[s] = *reinterpret_cast<const fx4*>(a.part + (s * rows + fr) * a.D + d);
+        }
+        M = fmaxf(M, ls[s]);
+    }
+    const float mr = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int s = 0; s < FEW_SPLITS; ++s) {
+        const float wgt = exp2_f(ls[s] - mr);
+        W += wgt;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fmaf(wgt, y[s][j], x[j]);
+    }
+    const float inv = W == 0.f ? 0.f : 1.f / W;
+    const int64_t at = out_at(a, (int)(fr / a.R), (int)(fr % a.R)) + d;
+    put4<TY>(a.o, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    if (a.o32) put4<F32>(a.o32, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W);
+}
+
+// Many splits: a workgroup owns a row, its threads take four columns of every (256 / columns)-th split, so that one latency covers many
+// splits, and are summed in a fixed order.
 
 template <int TY>
 __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
@@ -876,7 +1142,7 @@ __global__ __launch_bounds__(256) void join_sum_kernel(const float* part, void* 
 }
 
 // ---- launches of one element type (defined in that type's unit) -------------------------------------------------------------------------
-template <int TY> int launch_fwd(const Args& a, int keyw, hipStream_t s);
+template <int TY> int launch_fwd(const Args& a, int few, hipStream_t s);
 template <int TY> int launch_join_fwd(const Args& a, hipStream_t s);
 template <int TY> int launch_bwd_dq(const Args& a, hipStream_t s);
 template <int TY> int launch_bwd_dkv(const Args& a, hipStream_t s);

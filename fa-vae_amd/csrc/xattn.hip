@@ -7,7 +7,7 @@ using namespace xattn;
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 struct Plan {
-    int keyw, tiles, nsplit, span;
+    int few, tiles, nsplit, span;          // few: 0 many rows, 1 up to 64, 2 up to 16 (forward)
 };
 
 // Splits the streamed axis (n elements, steps of `step`, no span under `least`) until about `want` workgroups run.
@@ -28,12 +28,12 @@ Plan plan_fwd(const favae_xattn_desc* d) {
     const bool f32 = d->dtype == F32;
     Plan p{};
     if (R <= 64) {
-        p.keyw = 1;
+        p.few = R <= 16 ? 2 : 1;
         p.tiles = (int)((R + 31) / 32);
-        split_axis(p.tiles * heads, d->Lk, f32 && dim_pad(d->D) > 64 ? 64 : 128, 256, 1024, p);
+        split_axis(p.tiles * heads, d->Lk, f32 && dim_pad(d->D) > 64 ? 64 : 128, 256, 512, p);
     } else {
         p.tiles = (int)((R + 127) / 128);
-        split_axis(p.tiles * heads, d->Lk, 64, 512, 512, p);
+        split_axis(p.tiles * heads, d->Lk, 64, 512, f32 && d->D > 64 ? 256 : 512, p);       // workgroups the chip holds
     }
     return p;
 }
@@ -87,7 +87,7 @@ void use(Args& a, const Plan& p) { a.tiles = p.tiles; a.nsplit = p.nsplit; a.spa
 int64_t rows_of(const favae_xattn_desc* d) { return (int64_t)d->B * d->H * d->Lq; }
 
 int run_fwd(int ty, const Args& a, const Plan& p, hipStream_t s) {
-    return ty == F32 ? launch_fwd<F32>(a, p.keyw, s) : ty == BF16 ? launch_fwd<BF16>(a, p.keyw, s) : launch_fwd<F16>(a, p.keyw, s);
+    return ty == F32 ? launch_fwd<F32>(a, p.few, s) : ty == BF16 ? launch_fwd<BF16>(a, p.few, s) : launch_fwd<F16>(a, p.few, s);
 }
 int run_join_fwd(int ty, const Args& a, hipStream_t s) {
     return ty == F32 ? launch_join_fwd<F32>(a, s) : ty == BF16 ? launch_join_fwd<BF16>(a, s) : launch_join_fwd<F16>(a, s);

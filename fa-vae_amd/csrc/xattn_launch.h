@@ -20,7 +20,17 @@ int go_fwd(const Args& a, hipStream_t s) {
     return FAVAE_OK;
 }
 template <int TY, int DP>
-int go_fwd_dp(const Args& a, int keyw, hipStream_t s) { return keyw ? go_fwd<TY, DP, true>(a, s) : go_fwd<TY, DP, false>(a, s); }
+int go_token(const Args& a, hipStream_t s) {
+    using C = TokCfg<TY, DP>;
+    if (int rc = ready(fwd_token_kernel<TY, DP>, C::LDS)) return rc;
+    FAVAE_KLAUNCH((fwd_token_kernel<TY, DP>), dim3((unsigned)a.nsplit * a.B * a.Hkv), dim3(C::NT), C::LDS, s, a);
+    FAVAE_CHECK_LAUNCH();
+    return FAVAE_OK;
+}
+template <int TY, int DP>
+int go_fwd_dp(const Args& a, int few, hipStream_t s) {
+    return few == 2 ? go_token<TY, DP>(a, s) : few ? go_fwd<TY, DP, true>(a, s) : go_fwd<TY, DP, false>(a, s);
+}
 template <int TY, int DP>
 int go_dq(const Args& a, hipStream_t s) {
     using C = DqCfg<TY, DP>;
@@ -38,9 +48,9 @@ int go_dkv(const Args& a, hipStream_t s) {
     return FAVAE_OK;
 }
 
-template <int TY> int launch_fwd(const Args& a, int keyw, hipStream_t s) {
-    return a.D <= 32 ? go_fwd_dp<TY, 32>(a, keyw, s) : a.D <= 64 ? go_fwd_dp<TY, 64>(a, keyw, s)
-         : a.D <= 96 ? go_fwd_dp<TY, 96>(a, keyw, s) : go_fwd_dp<TY, 128>(a, keyw, s);
+template <int TY> int launch_fwd(const Args& a, int few, hipStream_t s) {
+    return a.D <= 32 ? go_fwd_dp<TY, 32>(a, few, s) : a.D <= 64 ? go_fwd_dp<TY, 64>(a, few, s)
+         : a.D <= 96 ? go_fwd_dp<TY, 96>(a, few, s) : go_fwd_dp<TY, 128>(a, few, s);
 }
 template <int TY> int launch_bwd_dq(const Args& a, hipStream_t s) {
     return a.D <= 32 ? go_dq<TY, 32>(a, s) : a.D <= 64 ? go_dq<TY, 64>(a, s) : a.D <= 96 ? go_dq<TY, 96>(a, s) : go_dq<TY, 128>(a, s);
@@ -49,7 +59,10 @@ template <int TY> int launch_bwd_dkv(const Args& a, hipStream_t s) {
     return a.D <= 32 ? go_dkv<TY, 32>(a, s) : a.D <= 64 ? go_dkv<TY, 64>(a, s) : a.D <= 96 ? go_dkv<TY, 96>(a, s) : go_dkv<TY, 128>(a, s);
 }
 template <int TY> int launch_join_fwd(const Args& a, hipStream_t s) {
-    FAVAE_KLAUNCH((join_fwd_kernel<TY>), dim3((unsigned)(a.B * a.Hkv) * a.R), dim3(256), 0, s, a);
+    if (a.nsplit <= FEW_SPLITS) {
+        const int64_t n = (int64_t)a.B * a.Hkv * a.R * (a.D / 4);
+        FAVAE_KLAUNCH((join_few_kernel<TY>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    } else FAVAE_KLAUNCH((join_fwd_kernel<TY>), dim3((unsigned)(a.B * a.Hkv) * a.R), dim3(256), 0, s, a);
     FAVAE_CHECK_LAUNCH();
     return FAVAE_OK;
 }
