@@ -208,8 +208,14 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
+# the handle alone, without the Stream object around it (0.3 instead of 2.7 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device())
 
 
 _hook = None

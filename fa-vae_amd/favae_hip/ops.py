@@ -1867,12 +1867,13 @@ def _require_float_gpu(what, *tensors):
     """all on one GPU and of one supported element type"""
     t0 = tensors[0]
     for t in tensors:
+        if t.is_cuda and t.dtype is t0.dtype and t.dtype in _DTYPE_ID and t.device == t0.device:
+            continue
         if not t.is_cuda:
             raise RuntimeError("favae_hip ops run on MI355X only (%s got a tensor on %s); there is no CPU fallback" % (what, t.device))
         if t.dtype not in _DTYPE_ID:
             raise RuntimeError("%s takes fp32, bf16 or fp16 tensors (got %s)" % (what, t.dtype))
-        if t.device != t0.device or t.dtype != t0.dtype:
-            raise RuntimeError("%s: tensors differ in device or type (%s %s, %s %s)" % (what, t0.device, t0.dtype, t.device, t.dtype))
+        raise RuntimeError("%s: tensors differ in device or type (%s %s, %s %s)" % (what, t0.device, t0.dtype, t.device, t.dtype))
 
 
 def _on_device(fn, device, *args):
@@ -1922,27 +1923,27 @@ def _xattn_plan(q, k, v, pad, scale):
 
 def _xattn_fwd(q, k, v, pad, scale, with_grad):
     """-> out, out before its rounding, row log-sums (the last two only for a backward pass)"""
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = q.new_empty(q.shape)
     if q.numel() == 0 or k.shape[1] == 0:
         return out.zero_(), None, None
     d, nbytes, _ = _xattn_plan(q, k, v, pad, scale)
     o32 = lse = ws = None
     if with_grad:
-        o32 = out if out.dtype == torch.float32 else torch.empty(q.shape, dtype=torch.float32, device=q.device)
-        lse = torch.empty((q.shape[0] * q.shape[1] * q.shape[2],), dtype=torch.float32, device=q.device)
+        o32 = out if out.dtype is torch.float32 else q.new_empty(q.shape, dtype=torch.float32)
+        lse = q.new_empty((q.shape[0] * q.shape[1] * q.shape[2],), dtype=torch.float32)
     if nbytes:
         ws = workspace(nbytes, q.device)
-    call("favae_xattn_fwd", byref(d), ptr(q), ptr(k), ptr(v), ptr(pad), ptr(out), ptr(o32), ptr(lse), ptr(ws), nbytes)
+    call("favae_xattn_fwd", byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(pad), out.data_ptr(), ptr(o32), ptr(lse), ptr(ws), nbytes)
     return out, o32, lse
 
 
 def _xattn_bwd(q, k, v, pad, scale, o32, lse, dout, need_kv):
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if need_kv else None
-    dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if need_kv else None
+    dq = q.new_empty(q.shape)
+    dk, dv = (k.new_empty(k.shape), v.new_empty(v.shape)) if need_kv else (None, None)
     d, _, nbytes = _xattn_plan(q, k, v, pad, scale)
     ws = workspace(nbytes, q.device)
-    call("favae_xattn_bwd", byref(d), ptr(q), ptr(k), ptr(v), ptr(pad), ptr(o32), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv), ptr(ws), nbytes)
+    call("favae_xattn_bwd", byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), ptr(pad), o32.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+         dq.data_ptr(), ptr(dk), ptr(dv), ws.data_ptr(), nbytes)
     return dq, dk, dv
 
 
@@ -2022,21 +2023,23 @@ def _check_padding_idx(what, padding_idx, rows):
 
 def _embed_fwd(ids, weight, scale):
     V, C = weight.shape
-    out = torch.empty((*ids.shape, C), dtype=weight.dtype, device=weight.device)
+    out = weight.new_empty((*ids.shape, C))
     if out.numel():
-        call("favae_embed_fwd", ptr(ids), ids.dtype == torch.int64, ptr(weight), weight.stride(0), V, ptr(out), ids.numel(), C,
+        call("favae_embed_fwd", ids.data_ptr(), ids.dtype is torch.int64, weight.data_ptr(), weight.stride(0), V, out.data_ptr(), ids.numel(), C,
              _DTYPE_ID[weight.dtype], scale)
     return out
 
 
 def _embed_bwd(dout, ids, rows, scale, padding):
     C = dout.shape[-1]
-    dw = torch.empty((rows, C), dtype=dout.dtype, device=dout.device)
-    if dout.numel() == 0:
+    dw = dout.new_empty((rows, C))
+    T = ids.numel()
+    if T == 0:
         return dw.zero_()
-    ws = workspace(query("favae_embed_bwd_workspace", ids.numel(), rows, C), dout.device)
-    call("favae_embed_bwd", ptr(ids), ids.dtype == torch.int64, ptr(dout), ids.numel(), rows, C, _DTYPE_ID[dout.dtype], scale, padding,
-         ptr(dw), ptr(ws), ws.numel())
+    nbytes = query("favae_embed_bwd_workspace", T, rows, C)
+    ws = workspace(nbytes, dout.device)
+    call("favae_embed_bwd", ids.data_ptr(), ids.dtype is torch.int64, dout.data_ptr(), T, rows, C, _DTYPE_ID[dout.dtype], scale, padding,
+         dw.data_ptr(), ws.data_ptr(), nbytes)
     return dw
 
 
