@@ -13,6 +13,8 @@
 //     dropped ones are below 2^-24 of the operands' product: 2.7 x the rate of the fp32 matrix instruction.
 // Rows that share a key / value head are packed: row r = g * Lq + i is query i of the g-th head of the group.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace xattn {
@@ -325,14 +327,13 @@ __device__ __forceinline__ f32x16 start16(const float* bias, int half) {
     }
     return s;
 }
-template <int TY, int DP, int ROWS>
-__device__ __forceinline__ f32x16 scores(const short* t, int row0, const Frag<Ty<TY>::PL> (&b)[DP / 16], bool all, const float* bias, int lane) {
-    const Frag<Ty<TY>::PL> f = row_frag<TY, DP, ROWS>(t, row0, 0, lane);
+template <int TY, int DP, int ROWS, bool ALL>
+__device__ __forceinline__ f32x16 scores(const short* t, int row0, const Frag<Ty<TY>::PL> (&b)[DP / 16], const float* bias, int lane) {
     f32x16 s;
-    if (all) s = mma<TY>(f, b[0], zero16());
-    else s = mma<TY>(f, b[0], start16(bias, lane >> 5));
+    if constexpr (ALL) s = zero16();
+    else s = start16(bias, lane >> 5);
 #pragma unroll
-    for (int d = 1; d < DP / 16; ++d) s = mma<TY>(row_frag<TY, DP, ROWS>(t, row0, 16 * d, lane), b[d], s);
+    for (int d = 0; d < DP / 16; ++d) s = mma<TY>(row_frag<TY, DP, ROWS>(t, row0, 16 * d, lane), b[d], s);
     return s;
 }
 
@@ -428,8 +429,13 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         const int sub0 = KEYW ? w : 0;                                     // this wave's first group of 32 keys
         if (KEYW && w >= C::NW) continue;
         f32x16 s[C::KS];
+        if (all) {
 #pragma unroll
-        for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK>(kt, 32 * (sub0 + t), qf, all, bi + 32 * (sub0 + t), lane);
+            for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK, true>(kt, 32 * (sub0 + t), qf, bi, lane);
+        } else {
+#pragma unroll
+            for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK, false>(kt, 32 * (sub0 + t), qf, bi + 32 * (sub0 + t), lane);
+        }
         float mx = s[0][0];
 #pragma unroll
         for (int t = 0; t < C::KS; ++t)
@@ -877,10 +883,15 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
 #pragma unroll
         for (int t = 0; t < C::BK / 32; ++t) {
             if ((unsigned)(word >> (32 * t)) == 0) continue;
-            const f32x16 s = scores<TY, DP, C::BK>(kt, 32 * t, qf, all, bi + 32 * t, lane);
-            f32x16 dp = zero16();
+            f32x16 s, dp;
+            const auto both = [&](auto every) {
+                s = scores<TY, DP, C::BK, decltype(every)::value>(kt, 32 * t, qf, bi + 32 * t, lane);
+                dp = zero16();
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) dp = mma<TY>(row_frag<TY, DP, C::BK>(vt, 32 * t, 16 * d, lane), df[d], dp);
+                for (int d = 0; d < DP / 16; ++d) dp = mma<TY>(row_frag<TY, DP, C::BK>(vt, 32 * t, 16 * d, lane), df[d], dp);
+            };
+            if (all) both(std::true_type{});
+            else both(std::false_type{});
             float ds[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i] = exp2_f(fmaf(s[i], a.c, -ls)) * (dp[i] - delta);
@@ -916,7 +927,7 @@ template <int TY, int DP> struct DkvCfg {
     static constexpr int BR = TY == F32 || DP > 64 ? 32 : 64, NT = 256, KEYS = 128;
     static constexpr int WAVES = (TY == F32 && DP > 32) || DP == 128 ? 1 : 2;
     static constexpr int TILE = tile_len<TY, DP, BR>();
-    static constexpr int BUFS = bufs_of(TILE, WAVES);
+    static constexpr int BUFS = DP == 96 ? 1 : bufs_of(TILE, WAVES);
     static constexpr size_t LDS = 2 * TILE * BUFS * 2 + BUFS * 2 * BR * 4;
 };
 
@@ -925,7 +936,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
     using C = DkvCfg<TY, DP>;
     using T = Ty<TY>;
     extern __shared__ __attribute__((aligned(16))) short lds[];
-    float* const stat = reinterpret_cast<float*>(lds + 2 * C::TILE * C::BUFS);    // [BUFS][BR log-sums, BR deltas] of the tile's rows
+    float* const stat = reinterpret_cast<float*>(lds + 2 * C::TILE * C::BUFS);    // [BUFS][BR log-sums, BR negative deltas] of the tile's rows
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tile = id % a.tiles; id /= a.tiles;
@@ -956,7 +967,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
         }
         const int x = r + tid % C::BR;
         if (tid < C::BR) st = x < rend ? a.lse[(int64_t)bh * a.R + x] - T::PSHIFT : INFINITY;
-        else if (tid < 2 * C::BR) st = x < rend ? a.delta[(int64_t)bh * a.R + x] : 0.f;
+        else if (tid < 2 * C::BR) st = x < rend ? -a.delta[(int64_t)bh * a.R + x] : 0.f;
     };
     if (r0 < rend) fetch(r0);
 
@@ -983,12 +994,12 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
         if (!work) continue;
 #pragma unroll
         for (int t = 0; t < C::BR / 32; ++t) {
-            if (r + 32 * t >= rend) continue;
-            f32x16 s = zero16(), dp = zero16();
+            f32x16 s = zero16(), dp = start16(lsd + C::BR + 32 * t, half);     // dp - delta: the sums start at -delta
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) s = mma<TY>(row_frag<TY, DP, C::BR>(qt, 32 * t, 16 * d, lane), kf[d], s);
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) dp = mma<TY>(row_frag<TY, DP, C::BR>(dt, 32 * t, 16 * d, lane), vf[d], dp);
+            if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);      // no operand reads ahead across the steps: registers
             float p[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -1004,12 +1015,9 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
                     dv[d] = mma<TY>(col_frag<TY, DP, C::BR>(dt, 32 * t + 16, 32 * d, lane), p1, dv[d]);
                 }
             }
+            if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const fx4 de = *reinterpret_cast<const fx4*>(lsd + C::BR + 32 * t + 8 * g + 4 * half);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[4 * g + i] *= dp[4 * g + i] - de[i];
-            }
+            for (int i = 0; i < 16; ++i) p[i] *= dp[i];
             sc.fit(p, dk);
             const Frag<T::PL> d0 = make_frag<TY>(p), d1 = make_frag<TY>(p + 8);
 #pragma unroll
