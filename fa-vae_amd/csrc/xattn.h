@@ -312,7 +312,7 @@ __device__ __forceinline__ int last_key(const uint8_t* pad, int k0, int k1, int 
 }
 
 // two LDS buffers (one barrier a tile) where as many workgroups still fit a CU as its registers allow
-constexpr int bufs_of(int tile, int waves) { return 4 * tile * 2 <= (waves == 1 ? 150000 : 77000) ? 2 : 1; }
+constexpr int bufs_of(int tile, int waves, bool pre) { return pre && 4 * tile * 2 <= (waves == 1 ? 150000 : 77000) ? 2 : 1; }
 // keys of a tile that take part: bit j of word i is key 64 i + j
 template <int BK> constexpr unsigned long long all_keys() { return BK >= 64 ? ~0ull : (1ull << (BK & 63)) - 1; }
 
@@ -347,11 +347,12 @@ template <int TY, int DP, bool KEYW> struct FwdCfg {
     static constexpr int NT = 256;
     static constexpr int NW = KEYW && TY == F32 && DP > 64 ? 2 : 4;        // waves that compute: the planes of 128 keys of 96, 128 fp32 columns
     static constexpr int ROWS = KEYW ? 32 : 32 * NW;                       // do not fit LDS, there two waves only load
-    static constexpr int WAVES = (TY == F32 && DP > 64) || (KEYW && DP == 128) ? 1 : 2;   // a SIMD; also keeps accumulators out of the second register file
+    static constexpr bool PRE = !(TY == F32 && DP > 64 && !KEYW);         // the next tile is loaded under this one's products (registers allowing)
+    static constexpr int WAVES = KEYW && (TY == F32 ? DP > 64 : DP == 128) ? 1 : 2;       // a SIMD; also keeps accumulators out of the second register file
     static constexpr int BK = KEYW ? 32 * NW : TY == F32 ? 32 : 64;
     static constexpr int KS = KEYW ? 1 : BK / 32;
     static constexpr int TILE = tile_len<TY, DP, BK>();
-    static constexpr int BUFS = bufs_of(TILE, WAVES);
+    static constexpr int BUFS = bufs_of(TILE, WAVES, PRE);
     static constexpr int RED = KEYW ? NW * DP * 32 * 2 : 0;               // joined results (fp32, in 16-bit units), over the tiles
     static constexpr int LEN = 2 * TILE * BUFS > RED ? 2 * TILE * BUFS : RED;
     static constexpr size_t LDS = LEN * 2 + BUFS * BK * 4 + 64 * 4 * NW + 16;
@@ -391,7 +392,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
             pb[i] = 64 * i + lane < C::BK && j < kend ? (pad ? pad[j] : 0) : 1;
         }
     };
-    fetch(k0);                                                             // k0 < Lk; on its way while the mask is looked through
+    if (C::PRE) fetch(k0);                                                 // k0 < Lk; on its way while the mask is looked through
     const int row = tile * C::ROWS + (KEYW ? 0 : 32 * w) + (lane & 31);
     Frag<T::PL> qf[DP / 16];
     load_row<TY, DP>(row < a.R ? (const char*)a.q + row_at(a, bh, row, a.q_b, a.q_l, a.q_h) * T::ES : nullptr, a.D, lane, qf);
@@ -403,6 +404,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
 
     int buf = 0;
     for (int key = k0; key < kend; key += C::BK) {
+        if (!C::PRE) fetch(key);
         unsigned long long word[(C::BK + 63) / 64];                        // bit j: key j of the tile takes part
         bool all = true;
 #pragma unroll
@@ -423,7 +425,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         sk.store(kt, tid);
         sv.store(vt, tid);
         __syncthreads();
-        if (key + C::BK < kend) fetch(key + C::BK);
+        if (C::PRE && key + C::BK < kend) fetch(key + C::BK);
         if (C::BUFS == 2) buf ^= 1;
 
         const int sub0 = KEYW ? w : 0;                                     // this wave's first group of 32 keys
@@ -804,9 +806,10 @@ template <int TY, int NACC> struct DsScale {
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DqCfg {
     static constexpr int BK = TY == F32 || DP == 128 ? 32 : 64, NT = 256, ROWS = 128;
-    static constexpr int WAVES = TY == F32 && DP > 64 ? 1 : 2;
+    static constexpr bool PRE = !(TY == F32 && DP > 64);
+    static constexpr int WAVES = PRE ? 2 : 1;
     static constexpr int TILE = tile_len<TY, DP, BK>();
-    static constexpr int BUFS = bufs_of(TILE, WAVES);
+    static constexpr int BUFS = bufs_of(TILE, WAVES, PRE);
     static constexpr size_t LDS = 2 * TILE * BUFS * 2 + BUFS * BK * 4 + 16;
 };
 
@@ -836,7 +839,7 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
         const int j = key + lane;
         pb = lane < C::BK && j < kend ? (pad ? pad[j] : 0) : 1;
     };
-    fetch(k0);                                                             // k0 < Lk; on its way while the mask is looked through
+    if (C::PRE) fetch(k0);                                                             // k0 < Lk; on its way while the mask is looked through
     kend = last_key<C::NT>(pad, k0, kend, tid, red);
 
     const int row = tile * C::ROWS + 32 * w + (lane & 31);
@@ -863,6 +866,7 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
 
     int buf = 0;
     for (int key = k0; key < kend; key += C::BK) {
+        if (!C::PRE) fetch(key);
         const unsigned long long word = __builtin_amdgcn_ballot_w64(pb == 0);
         const bool all = word == all_keys<C::BK>();
         short* const kt = lds + buf * 2 * C::TILE;
@@ -878,7 +882,7 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
         sk.store(kt, tid);
         sv.store(vt, tid);
         __syncthreads();
-        if (key + C::BK < kend) fetch(key + C::BK);
+        if (C::PRE && key + C::BK < kend) fetch(key + C::BK);
         if (C::BUFS == 2) buf ^= 1;
 #pragma unroll
         for (int t = 0; t < C::BK / 32; ++t) {
@@ -925,9 +929,10 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DkvCfg {
     static constexpr int BR = TY == F32 || DP > 64 ? 32 : 64, NT = 256, KEYS = 128;
-    static constexpr int WAVES = (TY == F32 && DP > 32) || DP == 128 ? 1 : 2;
+    static constexpr bool PRE = !(TY == F32 && DP > 32);
+    static constexpr int WAVES = (TY == F32 && DP > 64) || DP == 128 ? 1 : 2;
     static constexpr int TILE = tile_len<TY, DP, BR>();
-    static constexpr int BUFS = DP == 96 ? 1 : bufs_of(TILE, WAVES);
+    static constexpr int BUFS = DP == 96 ? 1 : bufs_of(TILE, WAVES, PRE);
     static constexpr size_t LDS = 2 * TILE * BUFS * 2 + BUFS * 2 * BR * 4;
 };
 
@@ -969,7 +974,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
         if (tid < C::BR) st = x < rend ? a.lse[(int64_t)bh * a.R + x] - T::PSHIFT : INFINITY;
         else if (tid < 2 * C::BR) st = x < rend ? -a.delta[(int64_t)bh * a.R + x] : 0.f;
     };
-    if (r0 < rend) fetch(r0);
+    if (C::PRE && r0 < rend) fetch(r0);
 
     Frag<T::PL> kf[DP / 16], vf[DP / 16];
     load_row<TY, DP>(live ? (const char*)a.k + (b * a.k_b + key * a.k_l + kv * a.k_h) * T::ES : nullptr, a.D, lane, kf);
@@ -981,6 +986,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
 
     int buf = 0;
     for (int r = r0; r < rend; r += C::BR) {
+        if (!C::PRE) fetch(r);
         short* const qt = lds + buf * 2 * C::TILE;
         short* const dt = qt + C::TILE;
         float* const lsd = stat + buf * 2 * C::BR;
@@ -989,7 +995,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
         sd.store(dt, tid);
         if (tid < 2 * C::BR) lsd[tid] = st;
         __syncthreads();
-        if (r + C::BR < rend) fetch(r + C::BR);
+        if (C::PRE && r + C::BR < rend) fetch(r + C::BR);
         if (C::BUFS == 2) buf ^= 1;
         if (!work) continue;
 #pragma unroll

@@ -33,7 +33,7 @@ Plan plan_fwd(const favae_xattn_desc* d) {
         split_axis(p.tiles * heads, d->Lk, f32 && dim_pad(d->D) > 64 ? 64 : 128, 256, 512, p);
     } else {
         p.tiles = (int)((R + 127) / 128);
-        split_axis(p.tiles * heads, d->Lk, 64, 512, f32 && d->D > 64 ? 256 : 512, p);       // workgroups the chip holds
+        split_axis(p.tiles * heads, d->Lk, 64, 512, 512, p);                      // workgroups the chip holds
     }
     return p;
 }
