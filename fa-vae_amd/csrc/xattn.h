@@ -521,29 +521,48 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
             }
         }
     } else {
-        if (row >= a.R) return;
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
         const float ls = lt == 0.f ? -INFINITY : m * a.c + (__builtin_amdgcn_logf(lt) - T::FSHIFT);
         const int64_t flat = ((int64_t)split * a.B * a.Hkv + bh) * a.R + row;
-        if (half == 0) {
+        const bool in = row < a.R;
+        if (half == 0 && in) {
             if (a.nsplit > 1) a.part_lse[flat] = ls;
             else if (a.lse) a.lse[(int64_t)bh * a.R + row] = lt == 0.f ? INFINITY : ls;
         }
-        const int64_t at = a.nsplit > 1 ? flat * a.D : out_at(a, bh, row);
+        // 32-bit results: a lane's four consecutive columns are one 16-byte store
+        if (TY == F32 || a.nsplit > 1 || a.o32) {
+            float* const to = a.nsplit > 1 ? a.part : TY == F32 ? (float*)a.o : a.o32;
+            const int64_t at = a.nsplit > 1 ? flat * a.D : in ? out_at(a, bh, row) : 0;
 #pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
+            for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int d = 32 * t + 8 * g;
-                if (d >= a.D) continue;
-                const float x0 = o[t][4 * g] * inv, x1 = o[t][4 * g + 1] * inv, x2 = o[t][4 * g + 2] * inv, x3 = o[t][4 * g + 3] * inv;
-                if (a.nsplit > 1) {
-                    put4<F32>(a.part, at + d + 4 * half, x0, x1, x2, x3);
-                } else {
-                    put4<TY>(a.o, at + d + 4 * half, x0, x1, x2, x3);
-                    if (a.o32) put4<F32>(a.o32, at + d + 4 * half, x0, x1, x2, x3);
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * t + 8 * g;
+                    if (d < a.D && in) put4<F32>(to, at + d + 4 * half, o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv);
                 }
+        }
+        // 16-bit results: transposed through LDS (a wave's own 32 rows), so that eight lanes or more write a row's consecutive 16 bytes
+        if constexpr (TY != F32) {
+            if (a.nsplit > 1) return;
+            __syncthreads();                                                // every wave is done with the tiles
+            short* const mine = lds + w * 32 * DP;
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int r = lane & 31, c = 4 * t + g;
+                    *reinterpret_cast<uint2*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)) + 4 * half) =
+                        make_uint2(pack2<TY>(o[t][4 * g] * inv, o[t][4 * g + 1] * inv), pack2<TY>(o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv));
+                }
+            __syncthreads();
+            constexpr int CPR = DP / 8;
+#pragma unroll
+            for (int i = 0; i < 32 * CPR / 64; ++i) {
+                const int e = lane + 64 * i, r = e / CPR, c = e % CPR, rr = tile * C::ROWS + 32 * w + r;
+                if (rr < a.R && 8 * c < a.D)
+                    *reinterpret_cast<ux4*>((short*)a.o + out_at(a, bh, rr) + 8 * c) = *reinterpret_cast<const ux4*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)));
             }
+        }
     }
 }
 
