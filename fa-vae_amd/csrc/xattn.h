@@ -545,6 +545,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         if constexpr (TY != F32) {
             if (a.nsplit > 1) return;
             __syncthreads();                                                // every wave is done with the tiles
+            static_assert(4 * 32 * DP <= C::LEN, "the waves' rows fit");
             short* const mine = lds + w * 32 * DP;
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t)
@@ -562,6 +563,126 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
                 if (rr < a.R && 8 * c < a.D)
                     *reinterpret_cast<ux4*>((short*)a.o + out_at(a, bh, rr) + 8 * c) = *reinterpret_cast<const ux4*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)));
             }
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------------------------------------
+// Forward over few keys (a prompt): all of them stay in LDS and a workgroup goes through many row tiles, each wave by itself without a
+// barrier, the next tile's queries on their way.  One maximum per row, nothing is rescaled.  What is left is reading q and writing o.
+// -------------------------------------------------------------------------------------------------------------------------------------
+template <int TY, int DP> struct ShortCfg {
+    static constexpr int NT = 256, KEYS = TY == F32 ? 96 : 128, KT = KEYS / 32;
+    static constexpr bool OK = TY != F32 || DP <= 64;                      // two workgroups a CU
+    static constexpr int TILE = tile_len<TY, DP, KEYS>();
+    static constexpr int OUT = TY == F32 ? 0 : 4 * 32 * DP;                // 16-bit results on their way out, a wave's own 32 rows
+    static constexpr size_t LDS = (2 * TILE + OUT) * 2 + KEYS * 4 + 16;
+};
+
+template <int TY, int DP>
+__global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
+    using C = ShortCfg<TY, DP>;
+    using T = Ty<TY>;
+    extern __shared__ __attribute__((aligned(16))) short lds[];
+    short* const kt = lds;
+    short* const vt = lds + C::TILE;
+    short* const out = lds + 2 * C::TILE;
+    float* const bias = reinterpret_cast<float*>(out + C::OUT);
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const int id = xcd_remap(blockIdx.x, gridDim.x), bh = id / a.tiles, b = bh / a.Hkv, kv = bh % a.Hkv;
+    const int r0 = (id % a.tiles) * a.span, rend = min(a.R, r0 + a.span);  // this workgroup's rows; span is a multiple of 128
+    const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
+    {
+        Stage<TY, DP, C::KEYS, C::NT> sk, sv;
+        sk.load(tid, a.D, (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES, a.k_l * T::ES, a.Lk);
+        sv.load(tid, a.D, (const char*)a.v + (b * a.v_b + kv * a.v_h) * T::ES, a.v_l * T::ES, a.Lk);
+        const bool k0 = lane < a.Lk && !(pad && pad[lane]), k1 = 64 + lane < a.Lk && !(pad && pad[64 + lane]);
+        const unsigned long long w0 = __builtin_amdgcn_ballot_w64(k0), w1 = __builtin_amdgcn_ballot_w64(k1);
+        const auto keep = [&](int r) { return (bool)((r >= 64 ? w1 >> (r & 63) : w0 >> r) & 1ull); };
+        sk.blank(tid, keep);
+        sv.blank(tid, keep);
+        sk.store(kt, tid);
+        sv.store(vt, tid);
+        if (tid < C::KEYS) bias[tid] = keep(tid) ? 0.f : -INFINITY;
+    }
+    __syncthreads();
+    const int nk = (a.Lk + 31) / 32;                                       // groups of 32 keys; behind the last key: bias -infinity
+
+    const auto row_ptr = [&](int r) { return r < rend ? (const char*)a.q + row_at(a, bh, r, a.q_b, a.q_l, a.q_h) * T::ES : nullptr; };
+    Frag<T::PL> qf[DP / 16];
+    load_row<TY, DP>(row_ptr(r0 + 32 * w + (lane & 31)), a.D, lane, qf);
+    for (int rt = r0 + 32 * w; rt < rend; rt += 128) {
+        const int row = rt + (lane & 31);
+        const bool in = row < rend;
+        f32x16 s[C::KT];
+#pragma unroll
+        for (int t = 0; t < C::KT; ++t)
+            if (t < nk) s[t] = scores<TY, DP, C::KEYS, false>(kt, 32 * t, qf, bias + 32 * t, lane);
+        load_row<TY, DP>(row_ptr(row + 128), a.D, lane, qf);               // the next tile's, under what follows
+        float m = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < C::KT; ++t)
+            if (t < nk) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, s[t][i]);
+            }
+        m = fmaxf(m, other_half(m));
+        const float sh = T::PSHIFT - (m == -INFINITY ? 0.f : m * a.c);     // probabilities of at most 1: fp16 takes them times 2^15
+        float l = 0.f;
+        f32x16 o[DP / 32];
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) o[t] = zero16();
+#pragma unroll
+        for (int t = 0; t < C::KT; ++t)
+            if (t < nk) {
+                float p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = exp2_f(fmaf(s[t][i], a.c, sh));
+                    l += p[i];
+                }
+                const Frag<T::PL> p0 = make_frag<TY>(p), p1 = make_frag<TY>(p + 8);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    o[d] = mma<TY>(col_frag<TY, DP, C::KEYS>(vt, 32 * t, 32 * d, lane), p0, o[d]);
+                    o[d] = mma<TY>(col_frag<TY, DP, C::KEYS>(vt, 32 * t + 16, 32 * d, lane), p1, o[d]);
+                }
+            }
+        l += other_half(l);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (half == 0 && in && a.lse) a.lse[(int64_t)bh * a.R + row] = l == 0.f ? INFINITY : m * a.c + (__builtin_amdgcn_logf(l) - T::PSHIFT);
+        if (TY == F32 || a.o32) {
+            float* const to = TY == F32 ? (float*)a.o : a.o32;
+            const int64_t at = in ? out_at(a, bh, row) : 0;
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * t + 8 * g;
+                    if (d < a.D && in) put4<F32>(to, at + d + 4 * half, o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv);
+                }
+        }
+        if constexpr (TY != F32) {
+            short* const mine = out + w * 32 * DP;
+            __builtin_amdgcn_wave_barrier();                               // a wave's LDS accesses are served in order
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int r = lane & 31, c = 4 * t + g;
+                    *reinterpret_cast<uint2*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)) + 4 * half) =
+                        make_uint2(pack2<TY>(o[t][4 * g] * inv, o[t][4 * g + 1] * inv), pack2<TY>(o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv));
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            constexpr int CPR = DP / 8;
+#pragma unroll
+            for (int i = 0; i < 32 * CPR / 64; ++i) {
+                const int e = lane + 64 * i, r = e / CPR, c = e % CPR, rr = rt + r;
+                if (rr < rend && 8 * c < a.D)
+                    *reinterpret_cast<ux4*>((short*)a.o + out_at(a, bh, rr) + 8 * c) = *reinterpret_cast<const ux4*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
 }

@@ -7,7 +7,7 @@ using namespace xattn;
 int64_t up(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 struct Plan {
-    int few, tiles, nsplit, span;          // few: 0 many rows, 1 up to 64, 2 up to 16 (forward)
+    int few, tiles, nsplit, span;          // few: 0 many rows, 1 up to 64, 2 up to 16, 3 many rows over few keys (forward)
 };
 
 // Splits the streamed axis (n elements, steps of `step`, no span under `least`) until about `want` workgroups run.
@@ -31,6 +31,13 @@ Plan plan_fwd(const favae_xattn_desc* d) {
         p.few = R <= 16 ? 2 : 1;
         p.tiles = (int)((R + 31) / 32);
         split_axis(p.tiles * heads, d->Lk, f32 && dim_pad(d->D) > 64 ? 64 : 128, 256, 512, p);
+    } else if (d->Lk <= (f32 ? 96 : 128) && (!f32 || d->D <= 64)) {
+        p.few = 3;
+        const int64_t tiles = (R + 127) / 128, want = (512 + heads - 1) / heads, wgs = want < tiles ? want : tiles;   // two workgroups a CU
+        const int64_t span = (tiles + wgs - 1) / wgs;                      // row tiles of a workgroup
+        p.nsplit = 1;
+        p.span = (int)(span * 128);
+        p.tiles = (int)((tiles + span - 1) / span);
     } else {
         p.tiles = (int)((R + 127) / 128);
         split_axis(p.tiles * heads, d->Lk, 64, 512, 512, p);                      // workgroups the chip holds

@@ -28,7 +28,18 @@ int go_token(const Args& a, hipStream_t s) {
     return FAVAE_OK;
 }
 template <int TY, int DP>
+int go_short(const Args& a, hipStream_t s) {
+    using C = ShortCfg<TY, DP>;
+    if (int rc = ready(fwd_short_kernel<TY, DP>, C::LDS)) return rc;
+    FAVAE_KLAUNCH((fwd_short_kernel<TY, DP>), dim3((unsigned)a.tiles * a.B * a.Hkv), dim3(C::NT), C::LDS, s, a);
+    FAVAE_CHECK_LAUNCH();
+    return FAVAE_OK;
+}
+template <int TY, int DP>
 int go_fwd_dp(const Args& a, int few, hipStream_t s) {
+    if constexpr (ShortCfg<TY, DP>::OK) {
+        if (few == 3) return go_short<TY, DP>(a, s);
+    }
     return few == 2 ? go_token<TY, DP>(a, s) : few ? go_fwd<TY, DP, true>(a, s) : go_fwd<TY, DP, false>(a, s);
 }
 template <int TY, int DP>
