@@ -278,6 +278,14 @@ template <int TY> __device__ __forceinline__ float frag_at(const Frag<Ty<TY>::PL
     return x;
 }
 
+// what eight floats lose in the 16-bit fragment made of them, as a fragment
+template <int TY> __device__ __forceinline__ Frag<Ty<TY>::PL> rest_frag(const float* x, const Frag<Ty<TY>::PL>& f) {
+    float r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = x[j] - frag_at<TY>(f, j);
+    return make_frag<TY>(r);
+}
+
 // four consecutive elements
 template <int TY>
 __device__ __forceinline__ void put4(void* p, int64_t e, float a, float b, float c, float d) {
@@ -465,6 +473,14 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
             }
             pf[2 * t] = make_frag<TY>(p);
             pf[2 * t + 1] = make_frag<TY>(p + 8);
+            if constexpr (KEYW && TY != F32) {                             // few rows: the matrix pipe has time for what p loses in 16 bits
+                const Frag<T::PL> r0 = rest_frag<TY>(p, pf[0]), r1 = rest_frag<TY>(p + 8, pf[1]);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    o[d] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0, 32 * d, lane), r0, o[d]);
+                    o[d] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16, 32 * d, lane), r1, o[d]);
+                }
+            }
         }
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
@@ -858,8 +874,14 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
             l += p[i];
         }
         const Frag<T::PL> pf = make_frag<TY>(p);
+        Frag<T::PL> rest;
+        if constexpr (TY != F32) rest = rest_frag<TY>(p, pf);              // the matrix pipe has time for what p loses in 16 bits
 #pragma unroll
-        for (int t = 0; t < DP / 16; ++t) o[t] = mma16<TY>(col_frag16<TY, DP, C::BK>(vt, 32 * w, 16 * t, lane), pf, o[t]);
+        for (int t = 0; t < DP / 16; ++t) {
+            const Frag<T::PL> vf = col_frag16<TY, DP, C::BK>(vt, 32 * w, 16 * t, lane);
+            if constexpr (TY != F32) o[t] = mma16<TY>(vf, rest, o[t]);
+            o[t] = mma16<TY>(vf, pf, o[t]);
+        }
     }
 
     float lt = l + __shfl_xor(l, 16, 64);

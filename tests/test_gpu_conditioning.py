@@ -111,7 +111,8 @@ def mask_of(kind, B, Lk, seed):
 
 
 SHAPES = [(1, 1, 1, 1, 1, 8), (2, 1, 77, 4, 2, 64), (2, 5, 130, 4, 1, 40), (1, 33, 64, 2, 2, 32), (2, 129, 65, 3, 3, 96), (1, 257, 300, 2, 1, 128),
-          (3, 64, 31, 8, 2, 16), (1, 700, 129, 2, 2, 64), (2, 130, 1100, 2, 1, 72), (1, 3, 2500, 4, 2, 128), (1, 1, 4099, 4, 1, 104)]
+          (3, 64, 31, 8, 2, 16), (1, 700, 129, 2, 2, 64), (2, 130, 1100, 2, 1, 72), (1, 3, 2500, 4, 2, 128), (1, 1, 4099, 4, 1, 104),
+          (1, 20, 700, 2, 1, 128), (2, 30, 300, 1, 1, 96), (1, 150, 400, 2, 2, 96), (1, 16, 513, 3, 3, 32), (1, 140, 40, 1, 1, 8)]
 
 
 @pytest.mark.parametrize("dtype", list(DT))
