@@ -10,13 +10,28 @@ struct Plan {
     int few, tiles, nsplit, span;          // few: 0 many rows, 1 up to 64, 2 up to 16, 3 many rows over few keys (forward)
 };
 
-// Splits the streamed axis (n elements, steps of `step`, no span under `least`) until about `want` workgroups run.
-void split_axis(int64_t base, int64_t n, int step, int least, int64_t want, Plan& p) {
-    int64_t s = base >= want ? 1 : (want + base - 1) / base;
-    const int64_t most = n / least > 1 ? n / least : 1;
-    if (s > most) s = most;
-    if (s > MOST_SPLITS) s = MOST_SPLITS;
-    const int64_t span = up((n + s - 1) / s, step);
+// Splits the streamed axis of n elements into spans (multiples of 64, none under 128): the number of splits with the smallest estimate.
+// `base` workgroups exist without splits, `fit` of them run together on a CU, `tau` us is what one alone takes for 64 elements (and about
+// as much to start); two together take 1.5 times as long, three 1.7 times; a join takes 4 us and reads `bytes` a split at 7 TB/s.
+// Measured (us): fp32, 192 workgroups of 1500 keys x 64 columns: 104 in one span, 79 + 6 in 2, 83 + 6 in 3, 71 + 7 in 4, 75 + 10 in 8;
+// fp32, 40 of 5036 x 128: 801, 410 + 5, 283 + 5, 227 + 5, 124 + 5 in 8, 102 + 10 in 12; fp16, 288 of 515 x 80: 29, 28 + 8 in 2.
+void split_axis(int64_t base, int64_t n, int fit, double tau, double bytes, Plan& p) {
+    static const double together[4] = {0.0, 1.0, 1.5, 1.7};
+    const int64_t most = n / 128 < 1 ? 1 : n / 128 < MOST_SPLITS ? n / 128 : MOST_SPLITS, slots = 256 * (int64_t)fit;
+    double best = 0.0;
+    for (int64_t s = 1; s <= most && (s == 1 || base * s <= 4 * slots); s += 1 + s / 16) {
+        const int64_t span = up((n + s - 1) / s, 64), ns = (n + span - 1) / span, full = base * ns / slots, rest = base * ns % slots;
+        const double t = (span / 64 + 1) * tau * (full * together[fit] + together[(rest + 255) / 256]) + (ns > 1 ? 4.0 + ns * bytes / 7e6 : 0.0);
+        if (s > 1 && t >= best) continue;
+        best = t;
+        p.span = (int)span;
+        p.nsplit = (int)ns;
+    }
+}
+// about `want` workgroups instead: few rows over many keys, bound by the keys' bytes
+void split_even(int64_t base, int64_t n, int step, int least, int64_t want, Plan& p) {
+    const int64_t most = n / least < 1 ? 1 : n / least < MOST_SPLITS ? n / least : MOST_SPLITS, w = (want + base - 1) / base;
+    const int64_t s = w < most ? w : most, span = up((n + s - 1) / s, step);
     p.span = (int)span;
     p.nsplit = (int)((n + span - 1) / span);
 }
@@ -30,7 +45,7 @@ Plan plan_fwd(const favae_xattn_desc* d) {
     if (R <= 64) {
         p.few = R <= 16 ? 2 : 1;
         p.tiles = (int)((R + 31) / 32);
-        split_axis(p.tiles * heads, d->Lk, f32 && dim_pad(d->D) > 64 ? 64 : 128, 256, 512, p);
+        split_even(p.tiles * heads, d->Lk, f32 && dim_pad(d->D) > 64 ? 64 : 128, 256, 512, p);   // measured on 32 heads x 30011 keys: 256, 1024 are slower
     } else if (d->Lk <= (f32 ? 96 : 128) && (!f32 || d->D <= 64)) {
         p.few = 3;
         const int64_t tiles = (R + 127) / 128, want = (512 + heads - 1) / heads, wgs = want < tiles ? want : tiles;   // two workgroups a CU
@@ -40,22 +55,24 @@ Plan plan_fwd(const favae_xattn_desc* d) {
         p.tiles = (int)((tiles + span - 1) / span);
     } else {
         p.tiles = (int)((R + 127) / 128);
-        split_axis(p.tiles * heads, d->Lk, 64, 512, 512, p);                      // workgroups the chip holds
+        split_axis(p.tiles * heads, d->Lk, !f32 && d->D <= 64 ? 3 : 2, (f32 ? 2.2 : 0.6) * dim_pad(d->D) / 32, 4.0 * R * heads * d->D, p);
     }
     return p;
 }
 Plan plan_dq(const favae_xattn_desc* d) {
-    const int64_t R = (int64_t)d->H / d->Hkv * d->Lq;
+    const int64_t R = (int64_t)d->H / d->Hkv * d->Lq, heads = (int64_t)d->B * d->Hkv;
     Plan p{};
     p.tiles = (int)((R + 127) / 128);
-    split_axis((int64_t)p.tiles * d->B * d->Hkv, d->Lk, 64, 512, 512, p);
+    const bool f32 = d->dtype == F32;
+    split_axis(p.tiles * heads, d->Lk, f32 ? (d->D > 64 ? 1 : 2) : d->D <= 64 ? 3 : 2, (f32 ? 2.4 : 0.75) * dim_pad(d->D) / 32, 4.0 * R * heads * d->D, p);
     return p;
 }
 Plan plan_dkv(const favae_xattn_desc* d) {
-    const int64_t R = (int64_t)d->H / d->Hkv * d->Lq;
+    const int64_t R = (int64_t)d->H / d->Hkv * d->Lq, heads = (int64_t)d->B * d->Hkv;
     Plan p{};
     p.tiles = (d->Lk + 127) / 128;
-    split_axis((int64_t)p.tiles * d->B * d->Hkv, R, 64, 256, 512, p);
+    const bool f32 = d->dtype == F32;
+    split_axis(p.tiles * heads, R, (f32 && d->D > 64) || d->D > 96 ? 1 : 2, (f32 ? 3.9 : 1.1) * dim_pad(d->D) / 32, 8.0 * heads * d->Lk * d->D, p);
     return p;
 }
 
