@@ -316,25 +316,26 @@ constexpr int GROUP = 32;        // positions whose ids and tokens one load brin
 
 template <int TY, bool VEC>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const uint2* sorted, const unsigned* valid, const void* dout, void* dw, float* part,
-                                                        int C, int chunk, int nseg, float scale) {
+                                                        int64_t T, int C, int chunk, int nseg, float scale) {
     using P = Piece<TY, VEC>;
     const int lane = threadIdx.x & 63;
-    const int64_t n = *valid, u = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t c = u / nseg, p0 = c * chunk, p1 = p0 + chunk < n ? p0 + chunk : n;
+    const int64_t u = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t c = u / nseg, p0 = c * chunk;
     const int col = ((int)(u - c * nseg) * 64 + lane) * P::N;
+    if (p0 >= T) return;
+    uint2 e = sorted[p0 + lane < T ? p0 + lane : T - 1];                   // behind *valid: anything, not used
+    const unsigned prev = sorted[p0 > 0 ? p0 - 1 : 0].x;
+    const int64_t n = *valid, p1 = p0 + chunk < n ? p0 + chunk : n;
     if (p0 >= p1) return;
     const bool in = col < C;
-    unsigned prev = p0 > 0 ? sorted[p0 - 1].x : 0xffffffffu;               // 0xffffffff: no id, they are below 2^31
-    bool first = true, head = false;
+    bool head = p0 > 0 && prev == (unsigned)__builtin_amdgcn_readlane((int)e.x, 0);       // the first run came from the chunk before
     float acc[P::N];
 #pragma unroll
     for (int i = 0; i < P::N; ++i) acc[i] = 0.f;
     constexpr int AHEAD = 8;
     for (int64_t q0 = p0; q0 < p1; q0 += GROUP) {
-        uint2 e = make_uint2(0xffffffffu, 0u);
-        if (lane <= GROUP && q0 + lane < n) e = sorted[q0 + lane];
-        if (first) head = prev == (unsigned)__builtin_amdgcn_readlane((int)e.x, 0);      // the first run came from the chunk before
-        first = false;
+        if (q0 > p0) e = sorted[q0 + lane < T ? q0 + lane : T - 1];
+        if (q0 + lane >= n) e = make_uint2(0xffffffffu, 0u);               // no id: they are below 2^31
         const int m = p1 - q0 < GROUP ? (int)(p1 - q0) : GROUP;
         for (int j0 = 0; j0 < m; j0 += AHEAD) {
             P x[AHEAD];
@@ -470,8 +471,9 @@ Plan plan(int64_t T, int64_t V, int C) {
     p.nblk = (int)((T + tpb - 1) / tpb);
     p.passes = 1;
     while (p.passes < 4 && (V - 1) >> (8 * p.passes)) ++p.passes;
-    int64_t chunk = T / 4096 / 8 * 8;                                      // at most about 4096 chunks: a run that fills them all is joined by one wave
-    p.chunk = (int)(chunk < 32 ? 32 : chunk);
+    // positions of a wave: short ones while there are few (340 tokens: 8 instead of 32 take 8 -> 4 us), about 4096 chunks of many tokens
+    const int64_t few = T / 2048 / 8 * 8, many = T / 4096 / 8 * 8;
+    p.chunk = (int)(many > 32 ? many : few > 32 ? 32 : few < 8 ? 8 : few);
     p.chunks = (T + p.chunk - 1) / p.chunk;
     p.pairs = up16((size_t)T * 8);
     p.counts = 2 * p.pairs;
@@ -502,7 +504,7 @@ int go_sums(const uint2* sorted, const unsigned* valid, const void* dout, void* 
     const int per = 64 * Piece<TY, VEC>::N, nseg = (C + per - 1) / per;
     const int64_t blocks = (p.chunks * nseg + 3) / 4;
     if (blocks > 0x7fffffff) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);
-    FAVAE_KLAUNCH((embed_sum_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dout, dw, part, C, p.chunk, nseg, scale);
+    FAVAE_KLAUNCH((embed_sum_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dout, dw, part, T, C, p.chunk, nseg, scale);
     FAVAE_CHECK_LAUNCH();
     if (p.chunks > 1) {
         FAVAE_KLAUNCH((embed_join_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dw, (const float*)part, T, C, p.chunk,
