@@ -492,7 +492,7 @@ int go_fwd(const void* ids, int i64, const void* w, int64_t ws, int64_t V, void*
     const int cpr = C / Piece<TY, VEC>::N;
     const int rows = cpr >= 1024 ? 1 : 1024 / cpr;
     const int64_t blocks = (T + rows - 1) / rows;
-    if (blocks > 0x7fffffff) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);
+    if (blocks >= 1 << 24) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);         // 2^32 threads a launch
     if (i64) FAVAE_KLAUNCH((embed_fwd_kernel<TY, VEC, int64_t>), dim3((unsigned)blocks), dim3(256), 0, s, ids, w, ws, V, out, T, C, cpr, rows, scale);
     else FAVAE_KLAUNCH((embed_fwd_kernel<TY, VEC, int32_t>), dim3((unsigned)blocks), dim3(256), 0, s, ids, w, ws, V, out, T, C, cpr, rows, scale);
     FAVAE_CHECK_LAUNCH();
@@ -503,7 +503,7 @@ template <int TY, bool VEC>
 int go_sums(const uint2* sorted, const unsigned* valid, const void* dout, void* dw, float* part, int64_t T, int C, const Plan& p, float scale, hipStream_t s) {
     const int per = 64 * Piece<TY, VEC>::N, nseg = (C + per - 1) / per;
     const int64_t blocks = (p.chunks * nseg + 3) / 4;
-    if (blocks > 0x7fffffff) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);
+    if (blocks >= 1 << 24) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);
     FAVAE_KLAUNCH((embed_sum_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dout, dw, part, T, C, p.chunk, nseg, scale);
     FAVAE_CHECK_LAUNCH();
     if (p.chunks > 1) {

@@ -591,7 +591,7 @@ template <int TY, int DP> struct ShortCfg {
     static constexpr int NT = 256, KEYS = TY == F32 ? 96 : 128, KT = KEYS / 32;
     static constexpr bool OK = TY != F32 || DP <= 64;                      // two workgroups a CU
     static constexpr int TILE = tile_len<TY, DP, KEYS>();
-    static constexpr int OUT = TY == F32 ? 0 : 4 * 32 * DP;                // 16-bit results on their way out, a wave's own 32 rows
+    static constexpr int OUT = TY == F32 || DP == 128 ? 0 : 4 * 32 * DP;   // 16-bit results on their way out, a wave's own 32 rows (128: no room)
     static constexpr size_t LDS = (2 * TILE + OUT) * 2 + KEYS * 4 + 16;
 };
 
@@ -678,7 +678,16 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
                     if (d < a.D && in) put4<F32>(to, at + d + 4 * half, o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv);
                 }
         }
-        if constexpr (TY != F32) {
+        if constexpr (TY != F32 && C::OUT == 0) {
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * t + 8 * g;
+                    if (d < a.D && in)
+                        put4<TY>(a.o, out_at(a, bh, row) + d + 4 * half, o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv);
+                }
+        } else if constexpr (TY != F32) {
             short* const mine = out + w * 32 * DP;
             __builtin_amdgcn_wave_barrier();                               // a wave's LDS accesses are served in order
 #pragma unroll

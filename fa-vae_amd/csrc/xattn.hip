@@ -82,8 +82,7 @@ bool ok_desc(const favae_xattn_desc* d) {
     if (d->dtype < F32 || d->dtype > F16 || !(d->scale > 0.f) || !(d->scale < INFINITY)) return false;
     const int64_t R = (int64_t)d->H / d->Hkv * d->Lq, heads = (int64_t)d->B * d->Hkv;
     if (R > (1 << 30) || d->Lk > (1 << 30) || heads > (1 << 24)) return false;
-    const int64_t most = ((R + 31) / 32 + (d->Lk + 127) / 128) * heads;    // workgroups of a launch, before splits (which stop at 1024)
-    if (most > (1 << 30)) return false;
+    if (((R + 31) / 32 > (d->Lk + 127) / 128 ? (R + 31) / 32 : (d->Lk + 127) / 128) * heads >= (1 << 24)) return false;   // 2^32 threads a launch
     const int64_t unit = d->dtype == F32 ? 4 : 8;                          // 16-byte accesses
     for (int64_t s : {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh})
         if (s < 0 || s % unit) return false;
@@ -145,8 +144,10 @@ extern "C" int favae_xattn_fwd(const favae_xattn_desc* d, const void* q, const v
     Args a = args_of(d, q, k, v, key_padding_mask);
     use(a, p);
     a.o = o; a.o32 = o32; a.lse = lse;
-    a.part = (float*)ws;
-    a.part_lse = a.part + p.nsplit * rows_of(d) * d->D;
+    if (p.nsplit > 1) {
+        a.part = (float*)ws;
+        a.part_lse = a.part + p.nsplit * rows_of(d) * d->D;
+    }
     FAVAE_PROF_NOTE(4.0 * rows_of(d) * d->Lk * d->D, 0);
     if (int rc = run_fwd(d->dtype, a, p, (hipStream_t)stream)) return rc;
     return p.nsplit > 1 ? run_join_fwd(d->dtype, a, (hipStream_t)stream) : FAVAE_OK;
