@@ -3,6 +3,11 @@
 // Both are memory-bound: the forward pass is one gather; the gradient reads every row of dout once and writes every row of dW.
 // The gradient has no float atomics: a stable radix sort brings equal ids together (integer counts only, so its order is fixed), each
 // wave sums a run of sorted positions in fp32 registers, runs that cross a chunk's border are joined in chunk order by a last pass.
+// Sums are fp32 for every type; a result is rounded once.
+// Measured (times of the kernels alone; 64 K tokens):
+//   8192 x 256 fp32, uniform ids     forward 19 us, gradient 42: counts 5 + 4, scatters 7 + 7, sums 14 (5.3 TB/s), joins 4
+//   49999 x 768 bf16, 1 / rank ids   forward 30 us, gradient 63: counts and zeros 12 + 4, scatters 7 + 7, sums 26 (4.4 TB/s), joins 11
+// The four launches of the sort move under 3 MB: they are bound by launches and latencies, at least 3 us each.
 #include "common.h"
 
 namespace {
@@ -63,7 +68,7 @@ template <int TY, bool VEC> struct Piece {
 template <typename I> __device__ __forceinline__ int64_t id_at(const void* ids, int64_t t) { return (int64_t)((const I*)ids)[t]; }
 
 // A block takes `rows` tokens of `cpr` pieces each; four pieces of a thread are in flight.  An id outside [0, V) reads nothing and gives
-// NaN.  At 65536 x 1024 fp16 the launch moves 268 MB.
+// NaN.  Bound by the writes: 65536 tokens x 1024 fp16 out of 16384 rows (34 MB) are 168 MB in 29 us, 5.8 TB/s; one token 1.4 us.
 template <int TY, bool VEC, typename I>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* ids, const void* w, int64_t w_stride, int64_t V, void* out, int64_t T,
                                                         int C, int cpr, int rows, float scale) {
@@ -99,6 +104,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* ids, const v
 // counts, so nothing depends on the order of the LDS atomics).  Ids outside [0, V) and the padding id are left out; *valid = entries
 // that remain.  Up to SMALL tokens are sorted by one workgroup in LDS in one launch.
 constexpr int DIGITS = 256, SORT_BLOCKS = 256, BATCH = 1024, SMALL = 2048;
+__host__ __device__ constexpr int up4(int n) { return (n + 3) & ~3; }      // a digit's counts begin at 16 bytes
 
 template <typename I>
 __device__ __forceinline__ bool entry_of(const void* ids, int64_t t, int64_t V, int64_t padding, unsigned& key) {
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(256) void embed_count_kernel(const void* ids, const
             if (live) atomicAdd(&h[key >> (8 * pass) & 255u], 1u);
         }
         __syncthreads();
-        count[tid * nblk + blockIdx.x] = h[tid];
+        count[tid * up4(nblk) + blockIdx.x] = h[tid];
     }
     if (FIRST) clear_rows(dw, dw_bytes, 0);
 }
@@ -208,46 +214,55 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(const void* ids, con
                                                             int tpb, int nblk, int pass, const unsigned* count, unsigned* valid) {
     __shared__ Ranker rk;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, blk = blockIdx.x;
+    I id[4];
+    uint2 e[4];
+    const int64_t t0 = (int64_t)blk * tpb;
+    const auto fetch = [&](int64_t b0) {                                   // a batch's entries; the first one's are on their way under the counts
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t t = b0 + 256 * w + 64 * k + lane, at = t < T ? t : T - 1;
+            if constexpr (FIRST) id[k] = ((const I*)ids)[at];
+            else e[k] = in[at];
+        }
+    };
+    fetch(t0);
     // where this block's entries of digit `tid` begin: all smaller digits, and the same digit of the blocks before
     unsigned before = 0, total = 0;
-    const unsigned* c = count + (int64_t)tid * nblk;
-    int i = 0;
-    for (; i + 16 <= nblk; i += 16) {                                      // sixteen loads in flight
-        unsigned x[16];
+    const u32x4_t* const c = reinterpret_cast<const u32x4_t*>(count + (int64_t)tid * up4(nblk));
+    const int quads = up4(nblk) / 4;
+    for (int i = 0; i < quads; i += 16) {                                  // sixteen loads in flight: 64 blocks, one latency
+        u32x4_t x[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = c[i + j];
+        for (int j = 0; j < 16; ++j) x[j] = c[min(i + j, quads - 1)];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            before += i + j < blk ? x[j] : 0;
-            total += x[j];
-        }
-    }
-    for (; i < nblk; ++i) {
-        const unsigned x = c[i];
-        before += i < blk ? x : 0;
-        total += x;
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int of = 4 * (i + j) + k;                            // its block; behind the last one: anything
+                const unsigned n = x[j][k];
+                before += of < blk ? n : 0;
+                total += of < nblk ? n : 0;
+            }
     }
     unsigned all;
     rk.run[tid] = rk.before(total, &all) + before;
     if (FIRST && blk == 0 && tid == 0) *valid = all;
-    const int64_t n = FIRST ? T : (int64_t)all, t0 = (int64_t)blk * tpb, t1 = t0 + tpb < n ? t0 + tpb : n;
+    const int64_t n = FIRST ? T : (int64_t)all, t1 = t0 + tpb < n ? t0 + tpb : n;
     for (int64_t b0 = t0; b0 < t1; b0 += BATCH) {
+        if (b0 > t0) fetch(b0);
         unsigned key[4], idx[4];
         bool live[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int64_t t = b0 + 256 * w + 64 * k + lane;
             live[k] = t < t1;
-            key[k] = idx[k] = 0;
-            if (live[k]) {
-                if constexpr (FIRST) {
-                    live[k] = entry_of<I>(ids, t, V, padding, key[k]);
-                    idx[k] = (unsigned)t;
-                } else {
-                    const uint2 e = in[t];
-                    key[k] = e.x;
-                    idx[k] = e.y;
-                }
+            if constexpr (FIRST) {
+                live[k] = live[k] && (int64_t)id[k] >= 0 && (int64_t)id[k] < V && (int64_t)id[k] != padding;
+                key[k] = (unsigned)id[k];
+                idx[k] = (unsigned)t;
+            } else {
+                key[k] = e[k].x;
+                idx[k] = e[k].y;
             }
         }
         rk.batch(key, idx, live, 8 * pass, [&](unsigned to, unsigned k, unsigned t) { out[to] = make_uint2(k, t); });
@@ -374,17 +389,17 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const uint2* sorted, con
 
 // A run that starts in chunk c and goes on: its part there, then those of the chunks that follow.  A wave takes one run and 64 pieces of
 // columns; a run of more than LONG parts is summed by the four waves of its workgroup, a contiguous quarter each, added in order.
-constexpr int LONG = 16;
+constexpr int LONG = 16, JOIN = 4;       // JOIN: waves of a workgroup
 
 template <int TY, bool VEC>
-__global__ __launch_bounds__(256) void embed_join_kernel(const uint2* sorted, const unsigned* valid, void* dw, const float* part, int64_t T, int C,
+__global__ __launch_bounds__(64 * JOIN) void embed_join_kernel(const uint2* sorted, const unsigned* valid, void* dw, const float* part, int64_t T, int C,
                                                          int chunk, int64_t chunks, int nseg, float scale) {
     using P = Piece<TY, VEC>;
-    __shared__ float sums[4][64 * P::N];
-    __shared__ int64_t run_end[4];
-    __shared__ unsigned run_id[4];
+    __shared__ float sums[JOIN][64 * P::N];
+    __shared__ int64_t run_end[JOIN];
+    __shared__ unsigned run_id[JOIN];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t u0 = (int64_t)blockIdx.x * 4, u = u0 + w, c = u / nseg, p0 = c * chunk, p1 = p0 + chunk;
+    const int64_t u0 = (int64_t)blockIdx.x * JOIN, u = u0 + w, c = u / nseg, p0 = c * chunk, p1 = p0 + chunk;
     // one load for the ids around this chunk's borders and one for the first ids of the next 64 chunks (entries behind *valid hold anything)
     const int64_t near = lane == 0 ? p1 - 1 : lane == 1 ? p1 : lane == 2 ? p0 : p0 - 1, next = (c + 1 + lane) * chunk;
     const unsigned e = c < chunks && near >= 0 && near < T ? sorted[near].x : 0u, f = next < T ? sorted[next].x : 0u;
@@ -395,30 +410,44 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const uint2* sorted, co
     int64_t end = -1;                                                      // last chunk that holds a part of the run that starts here
     if (goes_on && !came) {
         end = c + __builtin_ctzll(~__builtin_amdgcn_ballot_w64(c + 1 + lane <= most && f == id) | 1ull << 63);
-        while (end == c + 63 || (end > c + 63 && (end - c) % 64 == 63)) {  // all of them: look further
-            const int64_t k = end + 1 + lane;
-            const unsigned long long has = __builtin_amdgcn_ballot_w64(k <= most && sorted[(k <= most ? k : most) * chunk].x == id);
-            const int run = has == ~0ull ? 64 : __builtin_ctzll(~has);
-            end += run;
-            if (run < 64) break;
+        if (end == c + 63) {                                               // all of them: the last one by sixty-fourths of what follows
+            int64_t stop = most + 1;                                       // it is in [end, stop)
+            while (stop - end > 1) {
+                const int64_t step = (stop - end + 62) / 64, k = end + (lane + 1) * step;
+                const unsigned long long has = __builtin_amdgcn_ballot_w64(k < stop && sorted[(k < stop ? k : end) * chunk].x == id);
+                const int run = has == ~0ull ? 64 : __builtin_ctzll(~has);
+                stop = stop < end + (run + 1) * step ? stop : end + (run + 1) * step;
+                end += run * step;
+            }
         }
     }
     const int seg = (int)(u - c * nseg);
     const auto total = [&](int64_t cc, int64_t k0, int64_t k1, bool with_start, int col, float (&acc)[P::N]) {
-        const float* const at = part + (col < C ? col : 0);
 #pragma unroll
-        for (int j = 0; j < P::N; ++j) acc[j] = with_start ? at[(2 * cc + 1) * C + j] : 0.f;
+        for (int j = 0; j < P::N; ++j) acc[j] = with_start ? part[(2 * cc + 1) * C + (col < C ? col : 0) + j] : 0.f;
         constexpr int AHEAD = 8;
         for (int64_t k = k0; k <= k1; k += AHEAD) {
+            // no branch: all in flight; those behind k1 are out of the buffer's range, which reads zeros and moves nothing
+            const auto rs = make_rsrc(part + 2 * k * C, 0x7fffffffu);
             float x[AHEAD][P::N];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i)                                // no branch: all in flight
+            for (int i = 0; i < AHEAD; ++i) {
+                const unsigned at = k + i <= k1 && col < C ? 4u * (2u * i * (unsigned)C + (unsigned)col) : FAVAE_OOB;
+                if constexpr (VEC) {
 #pragma unroll
-                for (int j = 0; j < P::N; ++j) x[i][j] = at[2 * (k + i <= k1 ? k + i : k1) * C + j];
+                    for (int j = 0; j < P::N; j += 4) {
+                        const u32x4_t u = __builtin_amdgcn_raw_buffer_load_b128(rs, at + 4u * j, 0, 0);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) { const unsigned e = u[q]; x[i][j + q] = __builtin_bit_cast(float, e); }
+                    }
+                } else {
+                    x[i][0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0));
+                }
+            }
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-                for (int j = 0; j < P::N; ++j) acc[j] += k + i <= k1 ? x[i][j] : 0.f;
+                for (int j = 0; j < P::N; ++j) acc[j] += x[i][j];
         }
     };
     const bool is_long = end - c > LONG && end >= 0;
@@ -437,10 +466,10 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const uint2* sorted, co
         }
     }
     __syncthreads();
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < JOIN; ++i) {
         const int64_t last = run_end[i];
-        if (last < 0) continue;                                            // the same for all four waves
-        const int64_t uu = u0 + i, cc = uu / nseg, each = (last - cc + 3) / 4, k0 = cc + 1 + w * each, k1 = k0 + each - 1 < last ? k0 + each - 1 : last;
+        if (last < 0) continue;                                            // the same for all waves
+        const int64_t uu = u0 + i, cc = uu / nseg, each = (last - cc + JOIN - 1) / JOIN, k0 = cc + 1 + w * each, k1 = k0 + each - 1 < last ? k0 + each - 1 : last;
         const int col = ((int)(uu - cc * nseg) * 64 + lane) * P::N;
         P r;
         total(cc, k0, k1, w == 0, col, r.x);
@@ -449,7 +478,10 @@ __global__ __launch_bounds__(256) void embed_join_kernel(const uint2* sorted, co
         __syncthreads();
         if (w == 0 && col < C) {
 #pragma unroll
-            for (int j = 0; j < P::N; ++j) r.x[j] = (((r.x[j] + sums[1][64 * j + lane]) + sums[2][64 * j + lane]) + sums[3][64 * j + lane]) * scale;
+            for (int j = 0; j < P::N; ++j) {
+                for (int k = 1; k < JOIN; ++k) r.x[j] += sums[k][64 * j + lane];
+                r.x[j] *= scale;
+            }
             r.store(dw, (int64_t)run_id[i] * C + col);
         }
         __syncthreads();
@@ -477,7 +509,7 @@ Plan plan(int64_t T, int64_t V, int C) {
     p.chunks = (T + p.chunk - 1) / p.chunk;
     p.pairs = up16((size_t)T * 8);
     p.counts = 2 * p.pairs;
-    p.parts = p.counts + up16(((size_t)DIGITS * p.nblk + 4) * 4);
+    p.parts = p.counts + up16(((size_t)DIGITS * up4(p.nblk) + 4) * 4);
     p.total = p.parts + (size_t)p.chunks * 2 * C * 4;
     return p;
 }
@@ -490,7 +522,8 @@ bool vec_ok(int ty, int C, int64_t stride, const void* a, const void* b) {
 template <int TY, bool VEC>
 int go_fwd(const void* ids, int i64, const void* w, int64_t ws, int64_t V, void* out, int64_t T, int C, float scale, hipStream_t s) {
     const int cpr = C / Piece<TY, VEC>::N;
-    const int rows = cpr >= 1024 ? 1 : 1024 / cpr;
+    const int64_t least = (T >> 23) + 1;                                   // more rows a block where there are more than 2^23 of them
+    const int rows = (int)(cpr >= 1024 || 1024 / cpr < least ? least : 1024 / cpr);
     const int64_t blocks = (T + rows - 1) / rows;
     if (blocks >= 1 << 24) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);         // 2^32 threads a launch
     if (i64) FAVAE_KLAUNCH((embed_fwd_kernel<TY, VEC, int64_t>), dim3((unsigned)blocks), dim3(256), 0, s, ids, w, ws, V, out, T, C, cpr, rows, scale);
@@ -507,7 +540,7 @@ int go_sums(const uint2* sorted, const unsigned* valid, const void* dout, void* 
     FAVAE_KLAUNCH((embed_sum_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dout, dw, part, T, C, p.chunk, nseg, scale);
     FAVAE_CHECK_LAUNCH();
     if (p.chunks > 1) {
-        FAVAE_KLAUNCH((embed_join_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dw, (const float*)part, T, C, p.chunk,
+        FAVAE_KLAUNCH((embed_join_kernel<TY, VEC>), dim3((unsigned)((p.chunks * nseg + JOIN - 1) / JOIN)), dim3(64 * JOIN), 0, s, sorted, valid, dw, (const float*)part, T, C, p.chunk,
                       p.chunks, nseg, scale);
         FAVAE_CHECK_LAUNCH();
     }
@@ -548,7 +581,7 @@ extern "C" int favae_embed_bwd(const void* ids, int ids_are_64bit, const void* d
     const hipStream_t s = (hipStream_t)stream;
     uint2* const buf[2] = {(uint2*)ws, (uint2*)((char*)ws + p.pairs)};
     unsigned* const count = (unsigned*)((char*)ws + p.counts);
-    unsigned* const valid = count + (size_t)DIGITS * p.nblk;
+    unsigned* const valid = count + (size_t)DIGITS * up4(p.nblk);
     float* const part = (float*)((char*)ws + p.parts);
     const int64_t dw_bytes = V * C * (dtype == F32 ? 4 : 2);
     const int64_t zb = (dw_bytes + 65535) / 65536;                         // workgroups that clear the gradient

@@ -390,6 +390,18 @@ def test_one_id_for_all_tokens(T):
     assert not K.embedding_grad(do.to(DEV), ids.to(DEV), 9, 0.5, 5).any()        # all of them padding
 
 
+@pytest.mark.parametrize("C", [5, 64, 264])
+def test_runs_of_many_chunks(C):
+    """runs around 16, 64 and 128 chunks of 32 sorted tokens, which end at a chunk's border, one before or one behind it"""
+    K = ops()
+    lengths = [32 * n + x for n in (1, 2, 16, 17, 63, 64, 65, 128, 129, 200, 600) for x in (-1, 0, 1)]
+    ids = torch.repeat_interleave(torch.arange(len(lengths)) + 300, torch.tensor(lengths))      # two digits
+    ids = torch.cat([torch.zeros(130000 - len(ids), dtype=torch.long), ids])
+    ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(1))]
+    do = rnd((len(ids), C), 4, torch.float32)
+    emb_check(K.embedding_grad(do.to(DEV), ids.to(DEV), 400), ids, do, 400, 1.0, None, torch.float32)
+
+
 def test_order_of_equal_ids_is_fixed():
     """1, 2^24, -2^24, 1 in fp32 depends on its order: the sum runs over ascending tokens, every time"""
     K = ops()
