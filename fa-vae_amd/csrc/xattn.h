@@ -11,7 +11,12 @@
 //     the tile, and the transposed LDS read delivers the same order.  Probabilities never pass through LDS.
 //   * fp32 elements are split into three bf16 planes (24 significand bits, fp32's exponent range) and multiplied with six products, the
 //     dropped ones are below 2^-24 of the operands' product: 2.7 x the rate of the fp32 matrix instruction.
+//   * 16-bit elements: probabilities, and score gradients backward, are rounded to the element type for the second product: one MFMA
+//     instead of the two that a second plane would take, for half a step of the type per probability (results are then off by about 1.4
+//     times what the rounding of the result alone costs).  Sums, maxima, log-sums and accumulators are fp32.
 // Rows that share a key / value head are packed: row r = g * Lq + i is query i of the g-th head of the group.
+// Times at the kernels below are the kernel's alone, between the slowest and the fastest card measured; rates count 4, 6 and 8 D
+// operations a score for the forward pass, dq, and dk and dv.
 #pragma once
 #include <type_traits>
 
@@ -346,8 +351,15 @@ __device__ __forceinline__ f32x16 scores(const short* t, int row0, const Frag<Ty
 }
 
 // -------------------------------------------------------------------------------------------------------------------------------------
-// Forward.  KEYW = false: 4 waves of 32 rows each share 64 keys a tile.  KEYW = true, for few rows: one 32-row tile per workgroup,
-// each wave takes 32 other keys of the tile and the waves' results are joined at the end.
+// Forward: m = running maximum of s = q k^T, l = sum 2^(c s - c m), o = sum 2^(c s - c m) v / l.
+// KEYW = false: 4 waves of 32 rows each share 64 keys a tile (fp32: 32, its planes are three times as large).  KEYW = true, for 17 to 64
+// rows: one 32-row tile per workgroup, each wave takes 32 other keys of the tile and the waves' results are joined at the end.
+// Bound by the vector unit beside the matrix pipe: a 32 x 32 tile of 64 columns is 8 MFMAs and per lane 16 exponentials at a quarter of
+// the rate, 16 multiply-adds, maxima and sums and 8 packings; fp32 by its six products.  bf16, 64 heads x 4096 rows x 1024 keys x 64
+// columns: 101-118 us, 580-680 TFLOP/s.  fp32, 16 heads x 2048 x 2048 x 128: 205-227 us and 10 for the join of two spans, 150-168 TFLOP/s,
+// six times that on the matrix pipe.
+// One 32-row group a wave, 2 or 3 waves a SIMD: 64 rows a wave took the same time, two groups with interleaved exponentials 110, four
+// waves a SIMD 104-130 (spills), the next tile's stores between the products 15 % more.
 // -------------------------------------------------------------------------------------------------------------------------------------
 constexpr float LAZY = 8.f;      // the running maximum follows only when a row's scores exceed it by 2^8: p <= 2^8, few rescalings
 
@@ -586,6 +598,8 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
 // -------------------------------------------------------------------------------------------------------------------------------------
 // Forward over few keys (a prompt): all of them stay in LDS and a workgroup goes through many row tiles, each wave by itself without a
 // barrier, the next tile's queries on their way.  One maximum per row, nothing is rescaled.  What is left is reading q and writing o.
+// bf16, 128 heads x 4096 rows x 77 keys x 64 columns: 33 us, 4.1 TB/s of q and o (fwd_kernel: 46); fp32, 256 heads x 256 x 77 x 64: 20 us,
+// there each wave has one row tile and waits for the keys' planes.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct ShortCfg {
     static constexpr int NT = 256, KEYS = TY == F32 ? 96 : 128, KT = KEYS / 32;
@@ -716,7 +730,9 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
 // Forward of up to 16 rows a head group (a decoding step): bound by the bytes of K and V.  16x16x32 MFMAs hold the 16 rows in half the
 // registers of the 32-row form, so that two workgroups of 128 keys a tile share a CU and one's loads run under the other's arithmetic.
 // Each wave takes 32 keys of the tile: lane l holds row l % 16 and keys 4 (l / 16) + i and 16 + 4 (l / 16) + i, which are also the
-// contraction slots of the second product.
+// contraction slots of the second product.  fp16, 4 x 8 heads of 4 rows x 30011 keys x 128 columns in 16 spans: 87 us, 5.7 TB/s (32-row
+// form: 125), and 5 us for the join; bf16, 256 heads of one row x 77 keys: 6 us, of which a launch and two memory latencies are 4.
+// The matrix pipe has time here: probabilities are rounded to two planes, products of both are summed.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY> __device__ __forceinline__ fx4 mma16_1(s16x8 a, s16x8 b, fx4 c) {
     if constexpr (TY == F16)
@@ -974,6 +990,9 @@ template <int TY, int NACC> struct DsScale {
 // -------------------------------------------------------------------------------------------------------------------------------------
 // Backward, queries: delta = <dout, o>, dq = scale sum_j p (dp - delta) k.  4 waves of 32 rows, 64 keys a tile: scores and dp
 // transposed as in the forward pass (K and V rows are A operands), dq^T accumulates K^T ds^T.
+// Bound by both pipes: 12 MFMAs beside 16 exponentials, 32 multiply-adds and 8 packings per lane and tile of 64 columns.  bf16, 64 heads x
+// 4096 x 1024 x 64: 127-144 us, 715-810 TFLOP/s (dp started at -delta as in dk / dv: 136, its registers cost a wave a SIMD); fp16, 12 key
+// heads x 3063 rows x 515 x 80: 37 us, 288 workgroups on 256 CUs, 80 columns computed as 96; fp32, 256 x 256 x 77 x 64: 27 us.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DqCfg {
     static constexpr int BK = TY == F32 || DP == 128 ? 32 : 64, NT = 256, ROWS = 128;
@@ -1097,6 +1116,9 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
 // -------------------------------------------------------------------------------------------------------------------------------------
 // Backward, keys and values: 4 waves of 32 keys; the packed rows (all heads of the group, all queries) are streamed, 64 a tile.  Here a
 // lane owns a KEY: dk^T += Q^T ds, dv^T += dO^T p.  A padded key's column touches no other, so its result is simply written as zeros.
+// Bound by the matrix pipe and LDS: 16 MFMAs and 16 KB of LDS reads a wave and tile of 64 columns.  bf16, 64 heads x 4096 x 1024 x 64:
+// 151-174 us, 790-910 TFLOP/s (dp started at 0: 165; stores of the next tile between the products: 163); fp16, 12 key heads x 3063 rows x
+// 515 x 80 in 8 spans: 38 us and 5 for each join; fp32, 256 x 256 x 77 x 64: 39 us, registers leave no room for loads ahead.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DkvCfg {
     static constexpr int BR = TY == F32 || DP > 64 ? 32 : 64, NT = 256, KEYS = 128;
@@ -1230,7 +1252,8 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
 }
 
 // ---- joining splits -------------------------------------------------------------------------------------------------------------------
-// forward: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  Few splits: a thread owns four columns of a row.
+// forward: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  Few splits: a thread owns four columns of a row, bound by the partial
+// results' bytes (two splits of 32768 x 128 columns, 50 MB with the result: 10 us).
 constexpr int MOST_SPLITS = 1024, FEW_SPLITS = 8;
 
 template <int TY>
@@ -1268,8 +1291,7 @@ __global__ __launch_bounds__(256) void join_few_kernel(const Args a) {
 }
 
 // Many splits: a workgroup owns a row, its threads take four columns of every (256 / columns)-th split, so that one latency covers many
-// splits, and are summed in a fixed order.
-
+// splits, and are summed in a fixed order.  128 rows of 16 splits of 128 columns: 5 us, a launch and two latencies.
 template <int TY>
 __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
     __shared__ float wgt[MOST_SPLITS], part[256][4], red[8];
@@ -1312,7 +1334,7 @@ __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
     if (a.o32) put4<F32>(a.o32, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W);
 }
-// backward: out[i] = sum_s part[s][i], s ascending; n a multiple of 4
+// backward: out[i] = sum_s part[s][i], s ascending; n a multiple of 4.  8 splits of 0.5 M values: 5 us, about half of it the launch.
 template <int TY>
 __global__ __launch_bounds__(256) void join_sum_kernel(const float* part, void* out, int64_t n, int nsplit) {
     const int64_t e = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
