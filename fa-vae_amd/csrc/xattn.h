@@ -186,14 +186,22 @@ template <int TY, int DP, int ROWS, int NT> struct Stage {
     ux4 r[N];
     __device__ __forceinline__ static int row_of(int tid, int i) { return (tid + i * NT) / CPR; }
     __device__ __forceinline__ static int col_of(int tid, int i) { return (tid + i * NT) % CPR * Ty<TY>::EPC; }
-    // rows [0, rows) of the tile exist; rows >= 1
+    // rows [0, rows) of the tile exist; rows >= 1.  Chunk i of a thread lies i STEP rows behind its first one: the base moves, its offset stays
     __device__ __forceinline__ void load(int tid, int D, const char* base, int64_t stride, int rows) {
-        const int64_t bytes = rows * stride;
-        const auto rs = make_rsrc(base, (unsigned)(bytes < 0x7fffffff ? bytes : 0x7fffffff));
+        if constexpr (NT % CPR == 0) {
+            constexpr int STEP = NT / CPR;
+            const unsigned off = col_of(tid, 0) >= D ? FAVAE_OOB : (unsigned)row_of(tid, 0) * (unsigned)stride + col_of(tid, 0) * Ty<TY>::ES;
+            const int bytes = min(rows, ROWS) * (int)stride, step = STEP * (int)stride;    // under 2^31: at most 128 rows of 2^24 - 16
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const unsigned off = (unsigned)row_of(tid, i) * (unsigned)stride + col_of(tid, i) * Ty<TY>::ES;
-            r[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, col_of(tid, i) >= D || (PART && row_of(tid, i) >= ROWS) ? FAVAE_OOB : off, 0, 0);
+            for (int i = 0; i < N; ++i)
+                r[i] = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(base + i * step, (unsigned)max(bytes - i * step, 0)), off, 0, 0);
+        } else {
+            const auto rs = make_rsrc(base, (unsigned)min(rows, ROWS) * (unsigned)stride);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const unsigned off = (unsigned)row_of(tid, i) * (unsigned)stride + col_of(tid, i) * Ty<TY>::ES;
+                r[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, col_of(tid, i) >= D || (PART && row_of(tid, i) >= ROWS) ? FAVAE_OOB : off, 0, 0);
+            }
         }
     }
     // any rows: row_ptr(row) -> pointer to the row's elements or NULL (zeros instead)
@@ -214,7 +222,9 @@ template <int TY, int DP, int ROWS, int NT> struct Stage {
     __device__ __forceinline__ void blank(int tid, F keep) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const bool kp = (PART && row_of(tid, i) >= ROWS) || keep(row_of(tid, i));
+            int row = row_of(tid, i);
+            asm volatile("" : "+v"(row));                                  // computed here, where it is seldom needed: no registers in the loop
+            const bool kp = (PART && row >= ROWS) || keep(row);
 #pragma unroll
             for (int j = 0; j < 4; ++j) r[i][j] = kp ? r[i][j] : 0u;
         }
@@ -224,7 +234,9 @@ template <int TY, int DP, int ROWS, int NT> struct Stage {
         for (int i = 0; i < N; ++i) {
             const int row = row_of(tid, i), col = col_of(tid, i);
             if (PART && row >= ROWS) continue;
-            short* p = t + row * DP + 8 * ((col / 8) ^ swizzle<DP>(row)) + (col & 7);
+            // chunks a multiple of 16 rows apart: one address and constants
+            const int row0 = NT % (16 * CPR) == 0 ? row_of(tid, 0) : row, col0 = NT % (16 * CPR) == 0 ? col_of(tid, 0) : col;
+            short* p = t + row0 * DP + 8 * ((col0 / 8) ^ swizzle<DP>(row0)) + (col0 & 7) + (NT % (16 * CPR) == 0 ? i * (NT / CPR) * DP : 0);
             if constexpr (TY == F32) {
                 unsigned h0, m0, l0, h1, m1, l1;
                 const fx4 f = __builtin_bit_cast(fx4, r[i]);
@@ -306,6 +318,34 @@ __device__ __forceinline__ int64_t row_at(const Args& a, int bh, int r, int64_t 
 __device__ __forceinline__ int64_t out_at(const Args& a, int bh, int r) {
     return row_at(a, bh, r, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D);
 }
+// A wave's 32 packed rows from the wave-uniform r0 on: where they are of one head, which the longer axis makes the rule, row r0 + x lies
+// x strides behind the first (the division that finds the head is then made once for all 32, by scalars).
+struct Rows {
+    int r0;
+    int64_t first;                                       // element of row r0, or -1: several heads (or rows behind the last)
+    __device__ __forceinline__ Rows(const Args& a, int bh, int r, int64_t sb, int64_t sl, int64_t sh) {
+        r0 = __builtin_amdgcn_readfirstlane(r);
+        const int g = r0 / a.Lq, i = r0 - g * a.Lq;
+        first = r0 + 32 <= a.R && i + 32 <= a.Lq ? bh / a.Hkv * sb + i * sl + (int64_t)(bh % a.Hkv * a.G + g) * sh : -1;
+    }
+    __device__ __forceinline__ bool has(const Args& a, int x) const { return first >= 0 || r0 + x < a.R; }
+    // has(x)
+    __device__ __forceinline__ int64_t at(const Args& a, int bh, int x, int64_t sb, int64_t sl, int64_t sh) const {
+        return first >= 0 ? first + (unsigned)x * (unsigned)sl : row_at(a, bh, r0 + x, sb, sl, sh);
+    }
+};
+// a lane's row, r0 + lane % 32, of a tensor of TY; NULL behind the last one
+template <int TY>
+__device__ __forceinline__ const char* lane_row(const Args& a, const void* p, int bh, int r0, int lane, int64_t sb, int64_t sl, int64_t sh) {
+    const Rows rows(a, bh, r0, sb, sl, sh);
+    return rows.has(a, lane & 31) ? (const char*)p + rows.at(a, bh, lane & 31, sb, sl, sh) * Ty<TY>::ES : nullptr;
+}
+struct OutRows : Rows {
+    __device__ __forceinline__ OutRows(const Args& a, int bh, int r) : Rows(a, bh, r, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D) {}
+    __device__ __forceinline__ int64_t at(const Args& a, int bh, int x) const {
+        return Rows::at(a, bh, x, (int64_t)a.Lq * a.H * a.D, (int64_t)a.H * a.D, a.D);
+    }
+};
 
 // one behind the last key of [k0, k1) that is not padding (k0: there is none); every thread gets it.  `red`: one int of LDS.
 template <int NT>
@@ -319,15 +359,36 @@ __device__ __forceinline__ int last_key(const uint8_t* pad, int k0, int k1, int 
     for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
     if ((tid & 63) == 0) atomicMax(red, last);
     __syncthreads();
-    last = *red;
+    last = __builtin_amdgcn_readfirstlane(*red);
     __syncthreads();
     return last;
 }
 
 // two LDS buffers (one barrier a tile) where as many workgroups still fit a CU as its registers allow
 constexpr int bufs_of(int tile, int waves, bool pre) { return pre && 4 * tile * 2 <= (waves == 1 ? 150000 : 77000) ? 2 : 1; }
-// keys of a tile that take part: bit j of word i is key 64 i + j
-template <int BK> constexpr unsigned long long all_keys() { return BK >= 64 ? ~0ull : (1ull << (BK & 63)) - 1; }
+// keys of a tile that take part: bit j of word i is key 64 i + j.  The mask's bytes come a tile ahead, a byte a lane.
+template <int BK> struct KeyBits {
+    static constexpr int N = (BK + 63) / 64;
+    static constexpr unsigned long long ALL = BK >= 64 ? ~0ull : (1ull << (BK & 63)) - 1;
+    unsigned b[N];
+    __device__ __forceinline__ void load(const uint8_t* pad, int key, int kend, int lane) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            b[i] = 0;
+            if (pad) b[i] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(pad + key + 64 * i, (unsigned)max(0, min(64, kend - key - 64 * i))), lane, 0, 0);
+        }
+    }
+    __device__ __forceinline__ bool words(int left, unsigned long long (&word)[N]) const {      // left: keys from the tile's first on
+        bool all = true;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int n = min(left - 64 * i, min(64, BK - 64 * i));
+            word[i] = n <= 0 ? 0ull : __builtin_amdgcn_ballot_w64(b[i] == 0) & (~0ull >> (64 - n));
+            all = all && word[i] == ALL;
+        }
+        return all;
+    }
+};
 
 // key masks: a tile's scores start at 0 for a key and at -infinity for padding, as the accumulator of their first product
 __device__ __forceinline__ f32x16 start16(const float* bias, int half) {
@@ -368,7 +429,7 @@ template <int TY, int DP, bool KEYW> struct FwdCfg {
     static constexpr int NW = KEYW && TY == F32 && DP > 64 ? 2 : 4;        // waves that compute: the planes of 128 keys of 96, 128 fp32 columns
     static constexpr int ROWS = KEYW ? 32 : 32 * NW;                       // do not fit LDS, there two waves only load
     static constexpr bool PRE = !(TY == F32 && DP > 64 && !KEYW);         // the next tile is loaded under this one's products (registers allowing)
-    static constexpr int WAVES = KEYW && (TY == F32 ? DP > 64 : DP == 128) ? 1 : 2;       // a SIMD; also keeps accumulators out of the second register file
+    static constexpr int WAVES = KEYW && (TY == F32 ? DP > 64 : DP == 128) ? 1 : !KEYW && TY != F32 && DP <= 64 ? 3 : 2;       // a SIMD; also keeps accumulators out of the second register file
     static constexpr int BK = KEYW ? 32 * NW : TY == F32 ? 32 : 64;
     static constexpr int KS = KEYW ? 1 : BK / 32;
     static constexpr int TILE = tile_len<TY, DP, BK>();
@@ -402,20 +463,16 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
     int kend = min(a.Lk, k0 + a.span);
 
     Stage<TY, DP, C::BK, C::NT> sk, sv;
-    unsigned char pb[(C::BK + 63) / 64];
+    KeyBits<C::BK> pb;
     const auto fetch = [&](int key) {
         sk.load(tid, a.D, kp + key * a.k_l * T::ES, a.k_l * T::ES, kend - key);
         sv.load(tid, a.D, vp + key * a.v_l * T::ES, a.v_l * T::ES, kend - key);
-#pragma unroll
-        for (int i = 0; i < (C::BK + 63) / 64; ++i) {
-            const int j = key + 64 * i + lane;
-            pb[i] = 64 * i + lane < C::BK && j < kend ? (pad ? pad[j] : 0) : 1;
-        }
+        pb.load(pad, key, kend, lane);
     };
     if (C::PRE) fetch(k0);                                                 // k0 < Lk; on its way while the mask is looked through
-    const int row = tile * C::ROWS + (KEYW ? 0 : 32 * w) + (lane & 31);
+    const int row0 = tile * C::ROWS + (KEYW ? 0 : 32 * w), row = row0 + (lane & 31);
     Frag<T::PL> qf[DP / 16];
-    load_row<TY, DP>(row < a.R ? (const char*)a.q + row_at(a, bh, row, a.q_b, a.q_l, a.q_h) * T::ES : nullptr, a.D, lane, qf);
+    load_row<TY, DP>(lane_row<TY>(a, a.q, bh, row0, lane, a.q_b, a.q_l, a.q_h), a.D, lane, qf);
     kend = last_key<C::NT>(pad, k0, kend, tid, red);
     f32x16 o[DP / 32];
     float m = -INFINITY, l = 0.f;
@@ -425,19 +482,14 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
     int buf = 0;
     for (int key = k0; key < kend; key += C::BK) {
         if (!C::PRE) fetch(key);
-        unsigned long long word[(C::BK + 63) / 64];                        // bit j: key j of the tile takes part
-        bool all = true;
-#pragma unroll
-        for (int i = 0; i < (C::BK + 63) / 64; ++i) {
-            word[i] = __builtin_amdgcn_ballot_w64(pb[i] == 0);
-            all = all && word[i] == all_keys<C::BK>();
-        }
+        unsigned long long word[KeyBits<C::BK>::N];
+        const bool all = pb.words(kend - key, word);
         short* const kt = lds + buf * 2 * C::TILE;
         short* const vt = kt + C::TILE;
         float* const bi = bias + buf * C::BK;
         if (C::BUFS == 1) __syncthreads();
         if (!all) {
-            const auto keep = [&](int r) { return (bool)((C::BK > 64 && r >= 64 ? word[(C::BK + 63) / 64 - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
+            const auto keep = [&](int r) { return (bool)((C::BK > 64 && r >= 64 ? word[KeyBits<C::BK>::N - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
             sk.blank(tid, keep);
             sv.blank(tid, keep);
             if (tid < C::BK) bi[tid] = keep(tid) ? 0.f : -INFINITY;
@@ -457,6 +509,13 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         } else {
 #pragma unroll
             for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK, false>(kt, 32 * (sub0 + t), qf, bi + 32 * (sub0 + t), lane);
+        }
+        constexpr bool AHEAD = !KEYW && TY != F32 && DP <= 64;
+        Frag<T::PL> vf[2 * C::KS];
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int j = 0; j < 2 * C::KS; ++j) vf[j] = col_frag<TY, DP, C::BK>(vt, 16 * j, 0, lane);
+            __builtin_amdgcn_sched_barrier(0);
         }
         float mx = s[0][0];
 #pragma unroll
@@ -497,7 +556,17 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-            for (int j = 0; j < 2 * C::KS; ++j) o[t] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16 * j, 32 * t, lane), pf[j], o[t]);
+            for (int j = 0; j < 2 * C::KS; ++j) {
+                if constexpr (AHEAD) {
+                    o[t] = mma<TY>(vf[j], pf[j], o[t]);
+                    if (t + 1 < DP / 32) {
+                        vf[j] = col_frag<TY, DP, C::BK>(vt, 16 * j, 32 * (t + 1), lane);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
+                    o[t] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16 * j, 32 * t, lane), pf[j], o[t]);
+                }
+            }
     }
 
     const float lt = l + other_half(l);
@@ -553,6 +622,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         const float ls = lt == 0.f ? -INFINITY : m * a.c + (__builtin_amdgcn_logf(lt) - T::FSHIFT);
         const int64_t flat = ((int64_t)split * a.B * a.Hkv + bh) * a.R + row;
         const bool in = row < a.R;
+        const OutRows to_row(a, bh, row0);
         if (half == 0 && in) {
             if (a.nsplit > 1) a.part_lse[flat] = ls;
             else if (a.lse) a.lse[(int64_t)bh * a.R + row] = lt == 0.f ? INFINITY : ls;
@@ -560,7 +630,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         // 32-bit results: a lane's four consecutive columns are one 16-byte store
         if (TY == F32 || a.nsplit > 1 || a.o32) {
             float* const to = a.nsplit > 1 ? a.part : TY == F32 ? (float*)a.o : a.o32;
-            const int64_t at = a.nsplit > 1 ? flat * a.D : in ? out_at(a, bh, row) : 0;
+            const int64_t at = a.nsplit > 1 ? flat * a.D : in ? to_row.at(a, bh, lane & 31) : 0;
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
@@ -587,9 +657,9 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
             constexpr int CPR = DP / 8;
 #pragma unroll
             for (int i = 0; i < 32 * CPR / 64; ++i) {
-                const int e = lane + 64 * i, r = e / CPR, c = e % CPR, rr = tile * C::ROWS + 32 * w + r;
-                if (rr < a.R && 8 * c < a.D)
-                    *reinterpret_cast<ux4*>((short*)a.o + out_at(a, bh, rr) + 8 * c) = *reinterpret_cast<const ux4*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)));
+                const int e = lane + 64 * i, r = e / CPR, c = e % CPR;
+                if (to_row.has(a, r) && 8 * c < a.D)
+                    *reinterpret_cast<ux4*>((short*)a.o + to_row.at(a, bh, r) + 8 * c) = *reinterpret_cast<const ux4*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)));
             }
         }
     }
@@ -638,9 +708,9 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
     __syncthreads();
     const int nk = (a.Lk + 31) / 32;                                       // groups of 32 keys; behind the last key: bias -infinity
 
-    const auto row_ptr = [&](int r) { return r < rend ? (const char*)a.q + row_at(a, bh, r, a.q_b, a.q_l, a.q_h) * T::ES : nullptr; };
+    const auto row_ptr = [&](int rt) { return rt < rend ? lane_row<TY>(a, a.q, bh, rt, lane, a.q_b, a.q_l, a.q_h) : nullptr; };
     Frag<T::PL> qf[DP / 16];
-    load_row<TY, DP>(row_ptr(r0 + 32 * w + (lane & 31)), a.D, lane, qf);
+    load_row<TY, DP>(row_ptr(r0 + 32 * w), a.D, lane, qf);
     for (int rt = r0 + 32 * w; rt < rend; rt += 128) {
         const int row = rt + (lane & 31);
         const bool in = row < rend;
@@ -648,7 +718,7 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
 #pragma unroll
         for (int t = 0; t < C::KT; ++t)
             if (t < nk) s[t] = scores<TY, DP, C::KEYS, false>(kt, 32 * t, qf, bias + 32 * t, lane);
-        load_row<TY, DP>(row_ptr(row + 128), a.D, lane, qf);               // the next tile's, under what follows
+        load_row<TY, DP>(row_ptr(rt + 128), a.D, lane, qf);               // the next tile's, under what follows
         float m = -INFINITY;
 #pragma unroll
         for (int t = 0; t < C::KT; ++t)
@@ -680,10 +750,11 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
             }
         l += other_half(l);
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        const OutRows to_row(a, bh, rt);
         if (half == 0 && in && a.lse) a.lse[(int64_t)bh * a.R + row] = l == 0.f ? INFINITY : m * a.c + (__builtin_amdgcn_logf(l) - T::PSHIFT);
         if (TY == F32 || a.o32) {
             float* const to = TY == F32 ? (float*)a.o : a.o32;
-            const int64_t at = in ? out_at(a, bh, row) : 0;
+            const int64_t at = in ? to_row.at(a, bh, lane & 31) : 0;
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
@@ -699,7 +770,7 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
                 for (int g = 0; g < 4; ++g) {
                     const int d = 32 * t + 8 * g;
                     if (d < a.D && in)
-                        put4<TY>(a.o, out_at(a, bh, row) + d + 4 * half, o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv);
+                        put4<TY>(a.o, to_row.at(a, bh, lane & 31) + d + 4 * half, o[t][4 * g] * inv, o[t][4 * g + 1] * inv, o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv);
                 }
         } else if constexpr (TY != F32) {
             short* const mine = out + w * 32 * DP;
@@ -717,9 +788,9 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
             constexpr int CPR = DP / 8;
 #pragma unroll
             for (int i = 0; i < 32 * CPR / 64; ++i) {
-                const int e = lane + 64 * i, r = e / CPR, c = e % CPR, rr = rt + r;
-                if (rr < rend && 8 * c < a.D)
-                    *reinterpret_cast<ux4*>((short*)a.o + out_at(a, bh, rr) + 8 * c) = *reinterpret_cast<const ux4*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)));
+                const int e = lane + 64 * i, r = e / CPR, c = e % CPR;
+                if (to_row.has(a, r) && 8 * c < a.D)
+                    *reinterpret_cast<ux4*>((short*)a.o + to_row.at(a, bh, r) + 8 * c) = *reinterpret_cast<const ux4*>(mine + r * DP + 8 * (c ^ swizzle<DP>(r)));
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
@@ -810,15 +881,11 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
     int kend = min(a.Lk, k0 + a.span);
 
     Stage<TY, DP, C::BK, C::NT> sk, sv;
-    unsigned char pb[(C::BK + 63) / 64];
+    KeyBits<C::BK> pb;
     const auto fetch = [&](int key) {
         sk.load(tid, a.D, kp + key * a.k_l * T::ES, a.k_l * T::ES, kend - key);
         sv.load(tid, a.D, vp + key * a.v_l * T::ES, a.v_l * T::ES, kend - key);
-#pragma unroll
-        for (int i = 0; i < (C::BK + 63) / 64; ++i) {
-            const int j = key + 64 * i + lane;
-            pb[i] = j < kend ? (pad ? pad[j] : 0) : 1;
-        }
+        pb.load(pad, key, kend, lane);
     };
     fetch(k0);                                                             // k0 < Lk
     const int row = lane & 15;
@@ -851,16 +918,11 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
     for (int t = 0; t < DP / 16; ++t) o[t] = (fx4){0.f, 0.f, 0.f, 0.f};
 
     for (int key = k0; key < kend; key += C::BK) {
-        unsigned long long word[(C::BK + 63) / 64];
-        bool all = true;
-#pragma unroll
-        for (int i = 0; i < (C::BK + 63) / 64; ++i) {
-            word[i] = __builtin_amdgcn_ballot_w64(pb[i] == 0);
-            all = all && word[i] == ~0ull;
-        }
+        unsigned long long word[KeyBits<C::BK>::N];
+        const bool all = pb.words(kend - key, word);
         __syncthreads();
         if (!all) {
-            const auto keep = [&](int r) { return (bool)((r >= 64 ? word[(C::BK + 63) / 64 - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
+            const auto keep = [&](int r) { return (bool)((r >= 64 ? word[KeyBits<C::BK>::N - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
             sk.blank(tid, keep);
             sv.blank(tid, keep);
             if (tid < C::BK) bias[tid] = keep(tid) ? 0.f : -INFINITY;
@@ -1022,25 +1084,25 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
     int kend = min(a.Lk, k0 + a.span);
 
     Stage<TY, DP, C::BK, C::NT> sk, sv;
-    unsigned char pb;
+    KeyBits<C::BK> pb;
     const auto fetch = [&](int key) {
         sk.load(tid, a.D, kp + key * a.k_l * T::ES, a.k_l * T::ES, kend - key);
         sv.load(tid, a.D, vp + key * a.v_l * T::ES, a.v_l * T::ES, kend - key);
-        const int j = key + lane;
-        pb = lane < C::BK && j < kend ? (pad ? pad[j] : 0) : 1;
+        pb.load(pad, key, kend, lane);
     };
     if (C::PRE) fetch(k0);                                                             // k0 < Lk; on its way while the mask is looked through
     kend = last_key<C::NT>(pad, k0, kend, tid, red);
 
-    const int row = tile * C::ROWS + 32 * w + (lane & 31);
+    const int row0 = tile * C::ROWS + 32 * w, row = row0 + (lane & 31);
     const bool in = row < a.R;
+    const OutRows to_row(a, bh, row0);
     Frag<T::PL> qf[DP / 16], df[DP / 16];
-    load_row<TY, DP>(in ? (const char*)a.q + row_at(a, bh, row, a.q_b, a.q_l, a.q_h) * T::ES : nullptr, a.D, lane, qf);
-    load_row<TY, DP>(in ? (const char*)a.dout + row_at(a, bh, row, a.d_b, a.d_l, a.d_h) * T::ES : nullptr, a.D, lane, df);
+    load_row<TY, DP>(lane_row<TY>(a, a.q, bh, row0, lane, a.q_b, a.q_l, a.q_h), a.D, lane, qf);
+    load_row<TY, DP>(lane_row<TY>(a, a.dout, bh, row0, lane, a.d_b, a.d_l, a.d_h), a.D, lane, df);
     float delta = 0.f;
     {
         float g[DP / 16][8];
-        load_floats<DP>(in ? a.o32 + out_at(a, bh, row) : nullptr, a.D, lane, g);
+        load_floats<DP>(in ? a.o32 + to_row.at(a, bh, lane & 31) : nullptr, a.D, lane, g);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
@@ -1057,8 +1119,9 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
     int buf = 0;
     for (int key = k0; key < kend; key += C::BK) {
         if (!C::PRE) fetch(key);
-        const unsigned long long word = __builtin_amdgcn_ballot_w64(pb == 0);
-        const bool all = word == all_keys<C::BK>();
+        unsigned long long words[1];
+        const bool all = pb.words(kend - key, words);
+        const unsigned long long word = words[0];
         short* const kt = lds + buf * 2 * C::TILE;
         short* const vt = kt + C::TILE;
         float* const bi = bias + buf * C::BK;
@@ -1100,7 +1163,7 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
     }
     if (!in) return;
     const float inv = __builtin_ldexpf(a.scale, -(int)T::PSHIFT) / sc.f;
-    const int64_t at = a.nsplit > 1 ? (int64_t)split * a.B * a.Lq * a.H * a.D + out_at(a, bh, row) : out_at(a, bh, row);
+    const int64_t at = (a.nsplit > 1 ? (int64_t)split * a.B * a.Lq * a.H * a.D : 0) + to_row.at(a, bh, lane & 31);
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
@@ -1143,7 +1206,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
     const int key = tile * C::KEYS + 32 * w + (lane & 31);
     const bool in = key < a.Lk, live = in && !(a.pad && a.pad[b * a.pad_b + key]);
     const bool work = __builtin_amdgcn_ballot_w64(live) != 0;             // of this wave
-    const int r0 = split * a.span, rend = __syncthreads_or(work) ? min(a.R, r0 + a.span) : r0;
+    const int r0 = split * a.span, rend = __builtin_amdgcn_readfirstlane(__syncthreads_or(work)) ? min(a.R, r0 + a.span) : r0;
 
     Stage<TY, DP, C::BR, C::NT> sq, sd;
     float st = 0.f;

@@ -86,7 +86,9 @@ bool ok_desc(const favae_xattn_desc* d) {
     const int64_t unit = d->dtype == F32 ? 4 : 8;                          // 16-byte accesses
     for (int64_t s : {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh})
         if (s < 0 || s % unit) return false;
-    for (int64_t s : {d->q_sl, d->k_sl, d->v_sl})                          // rows follow one another and 128 of them span less than 2^31 bytes
+    // rows follow one another and 128 of them span less than 2^31 bytes (those of the dense outputs and of dout too)
+    if ((int64_t)d->H * d->D * (16 / unit) >= (1 << 24)) return false;
+    for (int64_t s : {d->q_sl, d->k_sl, d->v_sl})
         if (s < d->D || s * (16 / unit) >= (1 << 24)) return false;
     return true;
 }
