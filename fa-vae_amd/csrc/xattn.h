@@ -127,6 +127,10 @@ __device__ __forceinline__ f32x16 mma(const Frag<Ty<TY>::PL>& a, const Frag<Ty<T
     }
 }
 
+// a value that is the same for all lanes, in a scalar register: quotients are computed by the vector unit, and a buffer descriptor that
+// depends on one would be looped over
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
@@ -190,7 +194,8 @@ template <int TY, int DP, int ROWS, int NT> struct Stage {
     __device__ __forceinline__ void load(int tid, int D, const char* base, int64_t stride, int rows) {
         if constexpr (NT % CPR == 0) {
             constexpr int STEP = NT / CPR;
-            const unsigned off = col_of(tid, 0) >= D ? FAVAE_OOB : (unsigned)row_of(tid, 0) * (unsigned)stride + col_of(tid, 0) * Ty<TY>::ES;
+            // (no branch: one would turn the stride, and with it the descriptors, into lane values)
+            const unsigned off = ((unsigned)row_of(tid, 0) * (unsigned)stride + col_of(tid, 0) * Ty<TY>::ES) | (col_of(tid, 0) >= D ? FAVAE_OOB : 0u);
             const int bytes = min(rows, ROWS) * (int)stride, step = STEP * (int)stride;    // under 2^31: at most 128 rows of 2^24 - 16
 #pragma unroll
             for (int i = 0; i < N; ++i)
@@ -200,7 +205,7 @@ template <int TY, int DP, int ROWS, int NT> struct Stage {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const unsigned off = (unsigned)row_of(tid, i) * (unsigned)stride + col_of(tid, i) * Ty<TY>::ES;
-                r[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, col_of(tid, i) >= D || (PART && row_of(tid, i) >= ROWS) ? FAVAE_OOB : off, 0, 0);
+                r[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, off | (col_of(tid, i) >= D || (PART && row_of(tid, i) >= ROWS) ? FAVAE_OOB : 0u), 0, 0);
             }
         }
     }
@@ -325,7 +330,7 @@ struct Rows {
     int64_t first;                                       // element of row r0, or -1: several heads (or rows behind the last)
     __device__ __forceinline__ Rows(const Args& a, int bh, int r, int64_t sb, int64_t sl, int64_t sh) {
         r0 = __builtin_amdgcn_readfirstlane(r);
-        const int g = r0 / a.Lq, i = r0 - g * a.Lq;
+        const int g = uniform(r0 / a.Lq), i = r0 - g * a.Lq;
         first = r0 + 32 <= a.R && i + 32 <= a.Lq ? bh / a.Hkv * sb + i * sl + (int64_t)(bh % a.Hkv * a.G + g) * sh : -1;
     }
     __device__ __forceinline__ bool has(const Args& a, int x) const { return first >= 0 || r0 + x < a.R; }
@@ -375,7 +380,7 @@ template <int BK> struct KeyBits {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             b[i] = 0;
-            if (pad) b[i] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(pad + key + 64 * i, (unsigned)max(0, min(64, kend - key - 64 * i))), lane, 0, 0);
+            if (pad) b[i] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(pad + key + 64 * i, (unsigned)uniform(max(0, min(64, kend - key - 64 * i)))), lane, 0, 0);
         }
     }
     __device__ __forceinline__ bool words(int left, unsigned long long (&word)[N]) const {      // left: keys from the tile's first on
@@ -452,10 +457,10 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
     // keys), there the heads of a ragged batch alternate instead.
     int id = KEYW ? blockIdx.x : xcd_remap(blockIdx.x, gridDim.x);
     const int heads = a.B * a.Hkv;
-    const int bh = KEYW ? id % heads : id / (a.tiles * a.nsplit);
+    const int bh = uniform(KEYW ? id % heads : id / (a.tiles * a.nsplit));
     id = KEYW ? id / heads : id % (a.tiles * a.nsplit);
-    const int tile = id % a.tiles, split = id / a.tiles;
-    const int b = bh / a.Hkv, kv = bh % a.Hkv;
+    const int split = uniform(id / a.tiles), tile = uniform(id % a.tiles);
+    const int b = uniform(bh / a.Hkv), kv = bh - b * a.Hkv;
     const char* const kp = (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES;
     const char* const vp = (const char*)a.v + (b * a.v_b + kv * a.v_h) * T::ES;
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
@@ -689,8 +694,8 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
     short* const out = lds + 2 * C::TILE;
     float* const bias = reinterpret_cast<float*>(out + C::OUT);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    const int id = xcd_remap(blockIdx.x, gridDim.x), bh = id / a.tiles, b = bh / a.Hkv, kv = bh % a.Hkv;
-    const int r0 = (id % a.tiles) * a.span, rend = min(a.R, r0 + a.span);  // this workgroup's rows; span is a multiple of 128
+    const int id = xcd_remap(blockIdx.x, gridDim.x), bh = uniform(id / a.tiles), b = uniform(bh / a.Hkv), kv = bh - b * a.Hkv;
+    const int r0 = (id - bh * a.tiles) * a.span, rend = min(a.R, r0 + a.span);  // this workgroup's rows; span is a multiple of 128
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
     {
         Stage<TY, DP, C::KEYS, C::NT> sk, sv;
@@ -872,8 +877,8 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
     float* const stat = bias + C::BK;                                     // [2][NW][16] maxima, sums
     int* const red = reinterpret_cast<int*>(stat + 32 * C::NW);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
-    const int heads = a.B * a.Hkv, bh = blockIdx.x % heads, split = blockIdx.x / heads;   // heads alternate: a ragged batch is spread evenly
-    const int b = bh / a.Hkv, kv = bh % a.Hkv;
+    const int heads = a.B * a.Hkv, split = uniform(blockIdx.x / heads), bh = blockIdx.x - split * heads;   // heads alternate: a ragged batch is spread evenly
+    const int b = uniform(bh / a.Hkv), kv = bh - b * a.Hkv;
     const char* const kp = (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES;
     const char* const vp = (const char*)a.v + (b * a.v_b + kv * a.v_h) * T::ES;
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
@@ -1073,10 +1078,9 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
     float* const bias = reinterpret_cast<float*>(lds + 2 * C::TILE * C::BUFS);
     int* const red = reinterpret_cast<int*>(bias + C::BUFS * C::BK);
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int tile = id % a.tiles; id /= a.tiles;
-    const int split = id % a.nsplit, bh = id / a.nsplit;
-    const int b = bh / a.Hkv, kv = bh % a.Hkv;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int rest = uniform(id / a.tiles), tile = id - rest * a.tiles, bh = uniform(rest / a.nsplit), split = rest - bh * a.nsplit;
+    const int b = uniform(bh / a.Hkv), kv = bh - b * a.Hkv;
     const char* const kp = (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES;
     const char* const vp = (const char*)a.v + (b * a.v_b + kv * a.v_h) * T::ES;
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
@@ -1199,10 +1203,9 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
     extern __shared__ __attribute__((aligned(16))) short lds[];
     float* const stat = reinterpret_cast<float*>(lds + 2 * C::TILE * C::BUFS);    // [BUFS][BR log-sums, BR negative deltas] of the tile's rows
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int tile = id % a.tiles; id /= a.tiles;
-    const int split = id % a.nsplit, bh = id / a.nsplit;
-    const int b = bh / a.Hkv, kv = bh % a.Hkv;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int rest = uniform(id / a.tiles), tile = id - rest * a.tiles, bh = uniform(rest / a.nsplit), split = rest - bh * a.nsplit;
+    const int b = uniform(bh / a.Hkv), kv = bh - b * a.Hkv;
     const int key = tile * C::KEYS + 32 * w + (lane & 31);
     const bool in = key < a.Lk, live = in && !(a.pad && a.pad[b * a.pad_b + key]);
     const bool work = __builtin_amdgcn_ballot_w64(live) != 0;             // of this wave
@@ -1213,7 +1216,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
     const char* const qb = (const char*)a.q + (b * a.q_b + (int64_t)kv * a.G * a.q_h) * T::ES;
     const char* const db = (const char*)a.dout + (b * a.d_b + (int64_t)kv * a.G * a.d_h) * T::ES;
     const auto fetch = [&](int r) {
-        const int g0 = r / a.Lq, i0 = r - g0 * a.Lq, here = min(rend - r, a.Lq - i0);      // rows of head g0 from here on
+        const int g0 = uniform(r / a.Lq), i0 = r - g0 * a.Lq, here = min(rend - r, a.Lq - i0);      // rows of head g0 from here on
         if (here >= min(rend - r, C::BR)) {                                // the tile's rows are of one head
             sq.load(tid, a.D, qb + (i0 * a.q_l + g0 * a.q_h) * T::ES, a.q_l * T::ES, here);
             sd.load(tid, a.D, db + (i0 * a.d_l + g0 * a.d_h) * T::ES, a.d_l * T::ES, here);
