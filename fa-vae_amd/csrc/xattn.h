@@ -1065,10 +1065,9 @@ template <int TY, int NACC> struct DsScale {
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DqCfg {
     static constexpr int BK = TY == F32 || DP == 128 ? 32 : 64, NT = 256, ROWS = 128;
-    static constexpr bool PRE = !(TY == F32 && DP > 64);
-    static constexpr int WAVES = PRE ? 2 : 1;
+    static constexpr int WAVES = TY == F32 && DP > 64 ? 1 : 2;
     static constexpr int TILE = tile_len<TY, DP, BK>();
-    static constexpr int BUFS = bufs_of(TILE, WAVES, PRE);
+    static constexpr int BUFS = bufs_of(TILE, WAVES, true);
     static constexpr size_t LDS = 2 * TILE * BUFS * 2 + BUFS * BK * 4 + 16;
 };
 
@@ -1096,7 +1095,7 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
         sv.load(tid, a.D, vp + key * a.v_l * T::ES, a.v_l * T::ES, kend - key);
         pb.load(pad, key, kend, lane);
     };
-    if (C::PRE) fetch(k0);                                                             // k0 < Lk; on its way while the mask is looked through
+    fetch(k0);                                                             // k0 < Lk; on its way while the mask is looked through
     kend = last_key<C::NT>(pad, k0, kend, tid, red);
 
     const int row0 = tile * C::ROWS + 32 * w, row = row0 + (lane & 31);
@@ -1124,7 +1123,6 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
 
     int buf = 0;
     for (int key = k0; key < kend; key += C::BK) {
-        if (!C::PRE) fetch(key);
         unsigned long long words[1];
         const bool all = pb.words(kend - key, words);
         const unsigned long long word = words[0];
@@ -1141,7 +1139,7 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
         sk.store(kt, tid);
         sv.store(vt, tid);
         __syncthreads();
-        if (C::PRE && key + C::BK < kend) fetch(key + C::BK);
+        if (key + C::BK < kend) fetch(key + C::BK);
         if (C::BUFS == 2) buf ^= 1;
 #pragma unroll
         for (int t = 0; t < C::BK / 32; ++t) {
@@ -1187,15 +1185,19 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
 // lane owns a KEY: dk^T += Q^T ds, dv^T += dO^T p.  A padded key's column touches no other, so its result is simply written as zeros.
 // Bound by the matrix pipe and LDS: 16 MFMAs and 16 KB of LDS reads a wave and tile of 64 columns.  bf16, 64 heads x 4096 x 1024 x 64:
 // 144-175 us, 790-950 TFLOP/s (dp started at 0: 10 % more; stores of the next tile between the products: 8 %); fp16, 12 key heads x
-// 3063 rows x 515 x 80 in 8 spans: 38 us and 5 for each join; fp32, 256 x 256 x 77 x 64: 37 us, registers leave no room for loads ahead.
+// 3063 rows x 515 x 80 in 8 spans: 38 us and 5 for each join; fp32, 256 x 256 x 77 x 64: 37 us.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DkvCfg {
     static constexpr int BR = TY == F32 || DP > 64 ? 32 : 64, NT = 256, KEYS = 128;
-    static constexpr bool PRE = !(TY == F32 && DP > 32);
-    static constexpr int WAVES = (TY == F32 && DP > 64) || DP == 128 ? 1 : 2;
+    static constexpr bool TIGHT = DP > 64 || (TY == F32 && DP > 32);
+    static constexpr int WAVES = TY == F32 && DP > 64 ? 1 : 2;
+    // more than 64 columns (fp32: 32): the values' rows stay in LDS, their operands are read again for every tile, and dp is formed after
+    // the probabilities are used; a wave's registers hold no more beside both accumulators.  bf16, 64 heads x 1024 x 1024: 128 columns
+    // 148 -> 87 us (790 TFLOP/s, two waves a SIMD instead of one), 96 columns 87 -> 76 us; fp32 the same time within 2 %, without spills.
+    static constexpr int VALS = TIGHT ? tile_len<TY, DP, KEYS>() : 0;
     static constexpr int TILE = tile_len<TY, DP, BR>();
-    static constexpr int BUFS = DP == 96 ? 1 : bufs_of(TILE, WAVES, PRE);
-    static constexpr size_t LDS = 2 * TILE * BUFS * 2 + BUFS * 2 * BR * 4;
+    static constexpr int BUFS = TIGHT ? 1 : bufs_of(TILE, WAVES, true);
+    static constexpr size_t LDS = (2 * TILE * BUFS + VALS) * 2 + BUFS * 2 * BR * 4;
 };
 
 template <int TY, int DP>
@@ -1203,7 +1205,8 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
     using C = DkvCfg<TY, DP>;
     using T = Ty<TY>;
     extern __shared__ __attribute__((aligned(16))) short lds[];
-    float* const stat = reinterpret_cast<float*>(lds + 2 * C::TILE * C::BUFS);    // [BUFS][BR log-sums, BR negative deltas] of the tile's rows
+    short* const vals = lds + 2 * C::TILE * C::BUFS;
+    float* const stat = reinterpret_cast<float*>(vals + C::VALS);          // [BUFS][BR log-sums, BR negative deltas] of the tile's rows
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int rest = uniform(id / a.tiles), tile = id - rest * a.tiles, bh = uniform(rest / a.nsplit), split = rest - bh * a.nsplit;
@@ -1235,11 +1238,24 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
         if (tid < C::BR) st = x < rend ? a.lse[(int64_t)bh * a.R + x] - T::PSHIFT : INFINITY;
         else if (tid < 2 * C::BR) st = x < rend ? -a.delta[(int64_t)bh * a.R + x] : 0.f;
     };
-    if (C::PRE && r0 < rend) fetch(r0);
+    if (r0 < rend) fetch(r0);
 
-    Frag<T::PL> kf[DP / 16], vf[DP / 16];
+    Frag<T::PL> kf[DP / 16], vf[C::VALS ? 1 : DP / 16];
     load_row<TY, DP>(live ? (const char*)a.k + (b * a.k_b + key * a.k_l + kv * a.k_h) * T::ES : nullptr, a.D, lane, kf);
-    load_row<TY, DP>(live ? (const char*)a.v + (b * a.v_b + key * a.v_l + kv * a.v_h) * T::ES : nullptr, a.D, lane, vf);
+    if constexpr (C::VALS == 0) {
+        load_row<TY, DP>(live ? (const char*)a.v + (b * a.v_b + key * a.v_l + kv * a.v_h) * T::ES : nullptr, a.D, lane, vf);
+    } else if (r0 < rend) {
+        const int k0 = tile * C::KEYS, left = a.Lk - k0;
+        const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b + k0 : nullptr;
+        Stage<TY, DP, C::KEYS, C::NT> sv;
+        sv.load(tid, a.D, (const char*)a.v + (b * a.v_b + k0 * a.v_l + kv * a.v_h) * T::ES, a.v_l * T::ES, left);
+        if (pad) {
+            const unsigned long long w0 = __builtin_amdgcn_ballot_w64(lane < left && !pad[lane]);
+            const unsigned long long w1 = __builtin_amdgcn_ballot_w64(64 + lane < left && !pad[64 + lane]);
+            sv.blank(tid, [&](int r) { return (bool)((r >= 64 ? w1 >> (r & 63) : w0 >> (r & 63)) & 1ull); });
+        }
+        sv.store(vals, tid);                                               // the loop's barrier stands between this and the first read
+    }
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) dk[t] = dv[t] = zero16();
@@ -1247,7 +1263,6 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
 
     int buf = 0;
     for (int r = r0; r < rend; r += C::BR) {
-        if (!C::PRE) fetch(r);
         short* const qt = lds + buf * 2 * C::TILE;
         short* const dt = qt + C::TILE;
         float* const lsd = stat + buf * 2 * C::BR;
@@ -1256,17 +1271,24 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
         sd.store(dt, tid);
         if (tid < 2 * C::BR) lsd[tid] = st;
         __syncthreads();
-        if (C::PRE && r + C::BR < rend) fetch(r + C::BR);
+        if (r + C::BR < rend) fetch(r + C::BR);
         if (C::BUFS == 2) buf ^= 1;
         if (!work) continue;
 #pragma unroll
         for (int t = 0; t < C::BR / 32; ++t) {
-            f32x16 s = zero16(), dp = start16(lsd + C::BR + 32 * t, half);     // dp - delta: the sums start at -delta
+            f32x16 s = zero16(), dp;
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) s = mma<TY>(row_frag<TY, DP, C::BR>(qt, 32 * t, 16 * d, lane), kf[d], s);
+            const auto products = [&] {
+                dp = start16(lsd + C::BR + 32 * t, half);                  // dp - delta: the sums start at -delta
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) dp = mma<TY>(row_frag<TY, DP, C::BR>(dt, 32 * t, 16 * d, lane), vf[d], dp);
-            if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);      // no operand reads ahead across the steps: registers
+                for (int d = 0; d < DP / 16; ++d) {
+                    if constexpr (C::VALS == 0) dp = mma<TY>(row_frag<TY, DP, C::BR>(dt, 32 * t, 16 * d, lane), vf[d], dp);
+                    else dp = mma<TY>(row_frag<TY, DP, C::BR>(dt, 32 * t, 16 * d, lane), row_frag<TY, DP, C::KEYS>(vals, 32 * w, 16 * d, lane), dp);
+                }
+            };
+            if constexpr (!C::TIGHT) products();                            // beside the exponentials; registers have no room for both above
+            else __builtin_amdgcn_sched_barrier(0);
             float p[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -1282,7 +1304,11 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
                     dv[d] = mma<TY>(col_frag<TY, DP, C::BR>(dt, 32 * t + 16, 32 * d, lane), p1, dv[d]);
                 }
             }
-            if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (C::TIGHT) {
+                __builtin_amdgcn_sched_barrier(0);
+                products();
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) p[i] *= dp[i];
             sc.fit(p, dk);

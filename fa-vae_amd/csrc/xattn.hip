@@ -72,7 +72,7 @@ Plan plan_dkv(const favae_xattn_desc* d) {
     Plan p{};
     p.tiles = (d->Lk + 127) / 128;
     const bool f32 = d->dtype == F32;
-    split_axis(p.tiles * heads, R, (f32 && d->D > 64) || d->D > 96 ? 1 : 2, (f32 ? 3.9 : 1.1) * dim_pad(d->D) / 32, 8.0 * heads * d->Lk * d->D, p);
+    split_axis(p.tiles * heads, R, f32 && d->D > 64 ? 1 : 2, (f32 ? 3.9 : 1.1) * dim_pad(d->D) / 32, 8.0 * heads * d->Lk * d->D, p);
     return p;
 }
 
