@@ -126,3 +126,12 @@ def test_c_entry_points_refuse_before_they_launch():
               ebwd(T=1 << 31), ebwd(dw=P + 4), ebwd(ws=P + 8)):
         assert f == unsupported
     assert ebwd(n=lib.favae_embed_bwd_workspace(3, 4, 8) - 1) == workspace and lib.favae_embed_bwd_workspace(0, 4, 8) == 0
+
+
+def test_rows_of_very_many_heads_are_refused():
+    """the dense outputs' rows of H D elements have to stay under 2^24 bytes, whatever the strides of the inputs"""
+    lib = favae_hip.load()
+    for dtype, heads in ((0, 1 << 16), (1, 1 << 17)):                            # times 64 columns
+        at, under = (desc(B=1, Lq=1, Lk=1, H=h, Hkv=8, D=64, dtype=dtype) for h in (heads, heads - 8))
+        assert lib.favae_xattn_bwd_workspace(byref(at)) == 0 and lib.favae_xattn_bwd_workspace(byref(under)) > 0
+        assert lib.favae_xattn_fwd(byref(at), 1 << 12, 1 << 12, 1 << 12, None, 1 << 12, None, None, None, 0, None) == 3

@@ -157,6 +157,23 @@ def test_what_padded_rows_hold_reaches_nothing(dtype, Lq):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [40, 88, 128])
+def test_padded_tiles_between_live_ones(dtype, D):
+    """a tile of keys that is all padding between two that are not, and scattered padding in both: the bits of a run with zeros there"""
+    dt = DT[dtype]
+    B, Lq, Lk, H, Hkv = 2, 70, 300, 4, 2
+    q, k, v, do = rnd((B, Lq, H, D), 1, dt), rnd((B, Lk, Hkv, D), 2, dt), rnd((B, Lk, Hkv, D), 3, dt), rnd((B, Lq, H, D), 4, dt)
+    pad = mask_of("holes", B, Lk, 7)
+    pad[:, 128:256] = True
+    k[pad] = v[pad] = 0.0
+    clean = run(q, k, v, pad, D ** -0.5, do)
+    check(clean, *oracle(q, k, v, pad, D ** -0.5, do), dt)
+    k[pad], v[pad] = math.inf, math.nan
+    for n, t in run(q, k, v, pad, D ** -0.5, do).items():
+        assert torch.equal(t, clean[n]), n
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 def test_layouts_are_read_where_they_are(dtype):
     """views of a packed projection, head-major tensors, states shared by the batch, odd offsets: results of the dense copies, and gradients
     that go back through the views (a shared tensor's is the sum over its readers)"""
