@@ -1975,7 +1975,8 @@ def cross_attention(q, k, v, key_padding_mask=None, scale=None):
     """softmax(scale q k^T) v per head, where the keys and values come from another sequence than the queries (an encoder's states, a
     prompt), of another length.  q (B, Lq, H, D); k, v (B, Lk, Hkv, D) with H a multiple of Hkv: query head h reads key / value head
     h // (H // Hkv).  fp32, bf16 or fp16, all alike; D a multiple of 8 up to 128; any strides (views of a packed projection and expanded
-    tensors are read in place where their rows are contiguous and 16-byte aligned, other layouts are copied first).
+    tensors are read in place where their rows are contiguous and 16-byte aligned, other layouts are copied first); H * D values
+    under 16 MiB.
     key_padding_mask: bool (B, Lk), True = this key is padding (nn.MultiheadAttention's meaning); a row that is left without keys gives
     zeros, and whatever padded rows of k and v hold reaches no result.  scale: 1 / sqrt(D) unless given, positive.
     Lq = 1 (a decoding step) and long keys run the same call: the keys are split over the chip.  Differentiable in q, k, v, once."""
