@@ -422,8 +422,8 @@ __device__ __forceinline__ f32x16 scores(const short* t, int row0, const Frag<Ty
 // rows: one 32-row tile per workgroup, each wave takes 32 other keys of the tile and the waves' results are joined at the end.
 // Bound by issue: a 32 x 32 tile of 64 columns is 8 MFMAs and per lane 16 exponentials, multiply-adds, maxima / 2 and sums and 8 packings;
 // beside them addresses, waits and what a wave does once cost as much again, so every instruction counts (descriptors in scalars instead
-// of lane values: 118 -> 107 us).  bf16, 64 heads x 4096 rows x 1024 keys x 64 columns: 95-114 us, 600-720 TFLOP/s.  fp32 is bound by its
-// six products: 16 heads x 2048 x 2048 x 128 in two spans 181-195 us, 175-190 TFLOP/s, six times that on the matrix pipe; 10 us to join.
+// of lane values: 118 -> 107 us).  bf16, 64 heads x 4096 rows x 1024 keys x 64 columns: 95-118 us, 580-720 TFLOP/s.  fp32 is bound by its
+// six products: 16 heads x 2048 x 2048 x 128 in two spans 181-196 us, 175-190 TFLOP/s, six times that on the matrix pipe; 10 us to join.
 // One 32-row group a wave, 3 waves a SIMD with 16-bit elements of up to 64 columns (V's first half is read ahead of the exponentials: 3 %).
 // 64 rows a wave took the same time, two groups with interleaved exponentials 10 % more, four waves (32 keys at a time) 6 %, the next
 // tile's stores between the products 15 %, sums by products with ones 4 %.
@@ -1059,7 +1059,7 @@ template <int TY, int NACC> struct DsScale {
 // Backward, queries: delta = <dout, o>, dq = scale sum_j p (dp - delta) k.  4 waves of 32 rows, 64 keys a tile: scores and dp
 // transposed as in the forward pass (K and V rows are A operands), dq^T accumulates K^T ds^T.
 // Bound by both pipes: 12 MFMAs beside 16 exponentials, 32 multiply-adds and 8 packings per lane and tile of 64 columns.  bf16, 64 heads x
-// 4096 x 1024 x 64: 122-145 us, 710-850 TFLOP/s (both groups of 32 keys in one stretch of code, or dp started at -delta: 8-14 % more, their
+// 4096 x 1024 x 64: 122-147 us, 700-850 TFLOP/s (both groups of 32 keys in one stretch of code, or dp started at -delta: 8-14 % more, their
 // registers cost a wave a SIMD); fp16, 12 key heads x 3063 rows x 515 x 80: 37 us, 288 workgroups on 256 CUs, 80 columns computed as 96;
 // fp32, 256 x 256 x 77 x 64: 26 us.
 // -------------------------------------------------------------------------------------------------------------------------------------
@@ -1184,7 +1184,7 @@ __global__ __launch_bounds__(256, (DqCfg<TY, DP>::WAVES)) void bwd_dq_kernel(con
 // Backward, keys and values: 4 waves of 32 keys; the packed rows (all heads of the group, all queries) are streamed, 64 a tile.  Here a
 // lane owns a KEY: dk^T += Q^T ds, dv^T += dO^T p.  A padded key's column touches no other, so its result is simply written as zeros.
 // Bound by the matrix pipe and LDS: 16 MFMAs and 16 KB of LDS reads a wave and tile of 64 columns.  bf16, 64 heads x 4096 x 1024 x 64:
-// 144-175 us, 790-950 TFLOP/s (dp started at 0: 10 % more; stores of the next tile between the products: 8 %); fp16, 12 key heads x
+// 144-176 us, 780-950 TFLOP/s (dp started at 0: 10 % more; stores of the next tile between the products: 8 %); fp16, 12 key heads x
 // 3063 rows x 515 x 80 in 8 spans: 38 us and 5 for each join; fp32, 256 x 256 x 77 x 64: 37 us.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct DkvCfg {
