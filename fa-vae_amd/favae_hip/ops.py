@@ -1950,12 +1950,17 @@ def _xattn_bwd(q, k, v, pad, scale, o32, lse, dout, need_kv):
 class CrossAttentionFn(torch.autograd.Function):
     """Attention of one sequence's rows to another one's (cross_attention) with its backward pass.  Saved: the inputs, the output before
     its rounding (delta = <dout, out> of a rounded output would carry the rounding into every score gradient) and the row log-sums; the
-    probabilities are formed again.  Shared key / value heads: their gradients are summed over the group inside the kernel."""
+    probabilities are formed again.  Shared key / value heads: their gradients are summed over the group inside the kernel.
+    grad_mode: gradients are on where the call is made (within forward() they are off).  Whether the inputs need any is read here: a
+    traced program calls forward() again, with leaves where the traced inputs may have been plain."""
 
     @staticmethod
-    def forward(ctx, q, k, v, pad, scale):
+    def forward(ctx, q, k, v, pad, scale, grad_mode):
+        need = grad_mode and any(ctx.needs_input_grad)
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        out, o32, lse = _on_device(_xattn_fwd, q.device, q, k, v, pad, scale, True)
+        out, o32, lse = _on_device(_xattn_fwd, q.device, q, k, v, pad, scale, need)
+        if not need:
+            return out
         ctx.scale, ctx.same = scale, o32 is out
         ctx.save_for_backward(q, k, v, pad, out if ctx.same else o32, lse)
         return out
@@ -1965,10 +1970,10 @@ class CrossAttentionFn(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, pad, o32, lse = ctx.saved_tensors
         if lse is None:                                   # no row or no key: nothing depends on anything
-            return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)) + (None, None)
+            return tuple(torch.zeros(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)) + (None, None, None)
         need_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq, dk, dv = _on_device(_xattn_bwd, q.device, q, k, v, pad, ctx.scale, o32, lse, _dense16(dout), need_kv)
-        return dq, dk, dv, None, None
+        return dq, dk, dv, None, None, None
 
 
 def cross_attention(q, k, v, key_padding_mask=None, scale=None):
@@ -1979,7 +1984,8 @@ def cross_attention(q, k, v, key_padding_mask=None, scale=None):
     under 16 MiB.
     key_padding_mask: bool (B, Lk), True = this key is padding (nn.MultiheadAttention's meaning); a row that is left without keys gives
     zeros, and whatever padded rows of k and v hold reaches no result.  scale: 1 / sqrt(D) unless given, positive.
-    Lq = 1 (a decoding step) and long keys run the same call: the keys are split over the chip.  Differentiable in q, k, v, once."""
+    Lq = 1 (a decoding step) and long keys run the same call: the keys are split over the chip.  Differentiable in q, k, v, once and
+    backward: forward-mode tangents raise, as second derivatives do."""
     _require_float_gpu("cross_attention", q, k, v)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
         raise ValueError("cross_attention: q (B, Lq, H, D) and k, v (B, Lk, Hkv, D), got %s, %s, %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
@@ -2000,9 +2006,7 @@ def cross_attention(q, k, v, key_padding_mask=None, scale=None):
         if m.stride(1) != 1 and m.shape[1] > 1:
             m = m.contiguous()
         key_padding_mask = m
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return CrossAttentionFn.apply(q, k, v, key_padding_mask, scale)
-    return _on_device(_xattn_fwd, q.device, _rows16(q), _rows16(k), _rows16(v), key_padding_mask, scale, False)[0]
+    return CrossAttentionFn.apply(q, k, v, key_padding_mask, scale, torch.is_grad_enabled() or torch.jit.is_tracing())
 
 
 def _check_ids(what, ids, device):
@@ -2045,6 +2049,8 @@ def _embed_bwd(dout, ids, rows, scale, padding):
 
 
 class EmbeddingFn(torch.autograd.Function):
+    """Rows of a table by given ids (embedding); the backward pass is embedding_grad's"""
+
     @staticmethod
     def forward(ctx, weight, ids, scale, padding):
         ctx.rows, ctx.scale, ctx.padding = weight.shape[0], scale, padding
@@ -2061,7 +2067,8 @@ class EmbeddingFn(torch.autograd.Function):
 def embedding(ids, weight, scale=1.0, padding_idx=None):
     """scale * weight[ids]: ids (int64 or int32, any shape), weight (V, C) fp32, bf16 or fp16 -> (*ids.shape, C), one rounding.  The row
     padding_idx is looked up like any other and gets no gradient (nn.Embedding).  An id outside [0, V) reads nothing and gives a row of
-    NaN: ids stay on the device, so nothing can be raised without waiting for it.  Differentiable in weight, once (embedding_grad)."""
+    NaN: ids stay on the device, so nothing can be raised without waiting for it.  Differentiable in weight, once and backward
+    (embedding_grad): forward-mode tangents raise, as second derivatives do."""
     _require_float_gpu("embedding", weight)
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError("embedding: weight is (V, C), got %s" % (tuple(weight.shape),))
@@ -2070,9 +2077,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     scale = float(scale)
     if weight.stride(1) != 1 and weight.shape[1] > 1:
         weight = weight.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return EmbeddingFn.apply(weight, ids, scale, padding)
-    return _on_device(_embed_fwd, weight.device, ids, weight, scale)
+    return EmbeddingFn.apply(weight, ids, scale, padding)
 
 
 def embedding_grad(dout, ids, rows, scale=1.0, padding_idx=None):
