@@ -2064,6 +2064,18 @@ class EmbeddingFn(torch.autograd.Function):
         return _on_device(_embed_bwd, dout.device, _dense16(dout), ids, ctx.rows, ctx.scale, ctx.padding), None, None, None
 
 
+class EmbeddingGradFn(torch.autograd.Function):
+    """embedding_grad as a call of its own.  It is differentiable in nothing: a derivative that reaches it raises."""
+
+    @staticmethod
+    def forward(ctx, dout, ids, rows, scale, padding):
+        return _on_device(_embed_bwd, dout.device, _dense16(dout), ids, rows, scale, padding)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("embedding_grad is a gradient and has no derivative of its own")
+
+
 def embedding(ids, weight, scale=1.0, padding_idx=None):
     """scale * weight[ids]: ids (int64 or int32, any shape), weight (V, C) fp32, bf16 or fp16 -> (*ids.shape, C), one rounding.  The row
     padding_idx is looked up like any other and gets no gradient (nn.Embedding).  An id outside [0, V) reads nothing and gives a row of
@@ -2083,7 +2095,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
 def embedding_grad(dout, ids, rows, scale=1.0, padding_idx=None):
     """Gradient of embedding() with respect to its table of `rows` rows: (rows, C) with scale * the sum of dout[t] over ids[t] == v in row
     v (fp32 sums in a fixed order, rounded once), zeros where no token names the row or v == padding_idx.  Tokens are sorted by id
-    (stable); nothing is added atomically.  The call under embedding()'s backward pass, for programs that keep gradients themselves."""
+    (stable); nothing is added atomically.  The call under embedding()'s backward pass, for programs that keep gradients themselves; it has
+    no derivative, one that reaches it raises."""
     _require_float_gpu("embedding_grad", dout)
     rows = int(rows)
     if rows < 1 or dout.dim() < 1 or dout.shape[:-1] != ids.shape or dout.shape[-1] < 1:
@@ -2091,7 +2104,7 @@ def embedding_grad(dout, ids, rows, scale=1.0, padding_idx=None):
                          % (tuple(dout.shape), tuple(ids.shape), rows))
     ids = _check_ids("embedding_grad", ids, dout.device)
     padding = _check_padding_idx("embedding_grad", padding_idx, rows)
-    return _on_device(_embed_bwd, dout.device, _dense16(dout), ids, rows, float(scale), padding)
+    return EmbeddingGradFn.apply(dout, ids, rows, float(scale), padding)
 
 
 # ---------------------------------------------------------------------------------------------------------------

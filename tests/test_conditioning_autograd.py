@@ -1,4 +1,4 @@
-"""CPU: cross_attention and embedding stay visible to autograd and to the tracer whatever their inputs require, with the
+"""CPU: cross_attention, embedding and embedding_grad stay visible to autograd and to the tracer whatever their inputs require, with the
 launches stubbed: a launch fills its output with the number of the call."""
 import ctypes
 import warnings
@@ -61,6 +61,9 @@ def test_forward_mode_through_embedding_raises(launches):
         w = fwAD.make_dual(torch.randn(4, 8), torch.ones(4, 8))
         with pytest.raises(NotImplementedError, match="forward mode"):
             K.embedding(ids, w)
+        g = fwAD.make_dual(torch.randn(2, 2, 8), torch.ones(2, 2, 8))
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            K.embedding_grad(g, ids, 4)
 
 
 def traced(fn, *args):
@@ -72,8 +75,9 @@ def traced(fn, *args):
 def test_a_traced_program_launches(launches):
     """its results are those of its own launches, not the memory they would have been written to"""
     q, k, v = tensors()
-    ids, w = torch.tensor([0, 3, 1]), torch.randn(4, 8)
-    for fn, args in ((lambda q, k, v: K.cross_attention(q, k, v), (q, k, v)), (lambda ids, w: K.embedding(ids, w), (ids, w))):
+    ids, w, g = torch.tensor([0, 3, 1]), torch.randn(4, 8), torch.randn(3, 8)
+    for fn, args in ((lambda q, k, v: K.cross_attention(q, k, v), (q, k, v)), (lambda ids, w: K.embedding(ids, w), (ids, w)),
+                     (lambda g, ids: K.embedding_grad(g, ids, 4), (g, ids))):
         t = traced(fn, *args)
         for _ in range(2):
             n = len(launches)
@@ -95,6 +99,18 @@ def test_a_program_traced_without_gradients_has_them_later(launches):
     leaf = w.clone().requires_grad_()
     (dw,) = torch.autograd.grad(t(ids, leaf), leaf, torch.ones(3, 8))
     assert launches[-1] == "favae_embed_bwd" and bool((dw == len(launches)).all())
+
+
+def test_embedding_grad_keeps_its_history(launches):
+    """a gradient of a gradient is refused where it is asked for; the first derivative alone is not disturbed"""
+    ids = torch.tensor([0, 3, 1])
+    dw = K.embedding_grad(torch.randn(3, 8, requires_grad=True), ids, 4)
+    assert dw.requires_grad and bool((dw == 1.0).all())
+    with pytest.raises(RuntimeError, match="no derivative"):
+        dw.sum().backward()
+    assert not K.embedding_grad(torch.randn(3, 8), ids, 4).requires_grad
+    with torch.no_grad():
+        assert not K.embedding_grad(torch.randn(3, 8, requires_grad=True), ids, 4).requires_grad
 
 
 def test_nothing_is_kept_where_no_gradient_can_be_asked_for(launches, monkeypatch):

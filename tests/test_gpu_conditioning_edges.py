@@ -22,15 +22,17 @@ def test_traced_programs_give_the_eager_results():
     """with other values than the traced ones, and with leaves where the traced inputs were plain"""
     K = ops()
     q, k, v = (rnd(s, i, torch.float32).to(DEV) for i, s in enumerate(((2, 9, 4, 32), (2, 40, 2, 32), (2, 40, 2, 32))))
-    ids, w = torch.randint(0, 50, (3, 7)).to(DEV), rnd((50, 24), 4, torch.float32).to(DEV)
+    ids, w, g = torch.randint(0, 50, (3, 7)).to(DEV), rnd((50, 24), 4, torch.float32).to(DEV), rnd((3, 7, 24), 5, torch.float32).to(DEV)
     with warnings.catch_warnings():
         warnings.simplefilter("ignore")                                          # the checks of sizes are constants of a trace
         attend = torch.jit.trace(lambda q, k, v: K.cross_attention(q, k, v), (q, k, v), check_trace=False)
         embed = torch.jit.trace(lambda ids, w: K.embedding(ids, w, 2.0), (ids, w), check_trace=False)
+        grad = torch.jit.trace(lambda g, ids: K.embedding_grad(g, ids, 50), (g, ids), check_trace=False)
     for _ in range(3):
-        q, k, v, w = (t * -1.5 for t in (q, k, v, w))
+        q, k, v, w, g = (t * -1.5 for t in (q, k, v, w, g))
         ids = ids.add(1).remainder(50)
         assert torch.equal(attend(q, k, v), K.cross_attention(q, k, v)) and torch.equal(embed(ids, w), K.embedding(ids, w, 2.0))
+        assert torch.equal(grad(g, ids), K.embedding_grad(g, ids, 50))
         leaves = [t.clone().requires_grad_() for t in (q, k, v)]
         a, b = (torch.autograd.grad(f(*leaves), leaves, q) for f in (attend, K.cross_attention))
         assert all(torch.equal(x, y) for x, y in zip(a, b))
