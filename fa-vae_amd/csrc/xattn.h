@@ -73,17 +73,24 @@ __device__ __forceinline__ fx2 unpack2(unsigned u) {
     if constexpr (TY == F16) return __builtin_convertvector(__builtin_bit_cast(h16x2, u), fx2);
     else return (fx2){__builtin_bit_cast(float, u << 16), __builtin_bit_cast(float, u & 0xffff0000u)};
 }
-// x = hi + mid + lo, each rounded to nearest bf16.  An infinity stays in the first plane alone.
+// x = hi + mid + lo, each rounded to nearest bf16; values beyond bf16's largest have that one as hi, and the planes still add up to them.
+// An infinity stands in the last plane alone: mma() multiplies that plane by the other operand's first one only, which has its value's sign
+// and is 0 where the value is, so the product is the infinity (or the NaN) of the definition.  In the first plane it would also meet the
+// other's lower planes, whose signs say nothing.  PROB: probabilities, which are neither.
+template <bool PROB = false>
 __device__ __forceinline__ void split2(float a, float b, unsigned& hi, unsigned& mid, unsigned& lo) {
-    hi = pack2<BF16>(a, b);
+    constexpr float MOST = 0x1.fep127f;
+    const bool ia = !PROB && __builtin_isinf(a), ib = !PROB && __builtin_isinf(b);
+    const float fa = ia ? 0.f : a, fb = ib ? 0.f : b;
+    hi = PROB ? pack2<BF16>(a, b) : pack2<BF16>(__builtin_amdgcn_fmed3f(fa, -MOST, MOST), __builtin_amdgcn_fmed3f(fb, -MOST, MOST));
     const fx2 h = unpack2<BF16>(hi);
-    const float ra = __builtin_isinf(h.x) ? 0.f : a - h.x, rb = __builtin_isinf(h.y) ? 0.f : b - h.y;
+    const float ra = fa - h.x, rb = fb - h.y;                              // a NaN gets here, whatever the median made of it
     mid = pack2<BF16>(ra, rb);
     const fx2 m = unpack2<BF16>(mid);
-    lo = pack2<BF16>(ra - m.x, rb - m.y);
+    lo = pack2<BF16>(ia ? a : ra - m.x, ib ? b : rb - m.y);
 }
 // eight floats -> the planes of a fragment
-template <int TY>
+template <int TY, bool PROB = false>
 __device__ __forceinline__ Frag<Ty<TY>::PL> make_frag(const float* f) {
     Frag<Ty<TY>::PL> r;
     if constexpr (TY == F32) {
@@ -91,7 +98,7 @@ __device__ __forceinline__ Frag<Ty<TY>::PL> make_frag(const float* f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             unsigned a, b, c;
-            split2(f[2 * i], f[2 * i + 1], a, b, c);
+            split2<PROB>(f[2 * i], f[2 * i + 1], a, b, c);
             h[i] = a; m[i] = b; l[i] = c;
         }
         r.p[0] = __builtin_bit_cast(s16x8, h);
@@ -548,8 +555,8 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
                 p[i] = exp2_f(fmaf(s[t][i], a.c, sh));
                 l += p[i];
             }
-            pf[2 * t] = make_frag<TY>(p);
-            pf[2 * t + 1] = make_frag<TY>(p + 8);
+            pf[2 * t] = make_frag<TY, true>(p);
+            pf[2 * t + 1] = make_frag<TY, true>(p + 8);
             if constexpr (KEYW && TY != F32) {                             // few rows: the matrix pipe has time for what p loses in 16 bits
                 const Frag<T::PL> r0 = rest_frag<TY>(p, pf[0]), r1 = rest_frag<TY>(p + 8, pf[1]);
 #pragma unroll
@@ -747,7 +754,7 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
                     p[i] = exp2_f(fmaf(s[t][i], a.c, sh));
                     l += p[i];
                 }
-                const Frag<T::PL> p0 = make_frag<TY>(p), p1 = make_frag<TY>(p + 8);
+                const Frag<T::PL> p0 = make_frag<TY, true>(p), p1 = make_frag<TY, true>(p + 8);
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) {
                     o[d] = mma<TY>(col_frag<TY, DP, C::KEYS>(vt, 32 * t, 32 * d, lane), p0, o[d]);
@@ -966,7 +973,7 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
             p[i] = exp2_f(fmaf(s[i >> 2][i & 3], a.c, sh));
             l += p[i];
         }
-        const Frag<T::PL> pf = make_frag<TY>(p);
+        const Frag<T::PL> pf = make_frag<TY, true>(p);
         Frag<T::PL> rest;
         if constexpr (TY != F32) rest = rest_frag<TY>(p, pf);              // the matrix pipe has time for what p loses in 16 bits
 #pragma unroll
@@ -1297,7 +1304,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
                 for (int i = 0; i < 4; ++i) p[4 * g + i] = exp2_f(fmaf(s[4 * g + i], a.c, -ls[i]));
             }
             {
-                const Frag<T::PL> p0 = make_frag<TY>(p), p1 = make_frag<TY>(p + 8);
+                const Frag<T::PL> p0 = make_frag<TY, true>(p), p1 = make_frag<TY, true>(p + 8);
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) {
                     dv[d] = mma<TY>(col_frag<TY, DP, C::BR>(dt, 32 * t, 32 * d, lane), p0, dv[d]);

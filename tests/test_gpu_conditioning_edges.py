@@ -46,3 +46,79 @@ def test_a_call_without_gradients_gives_the_same_bits():
             q, k, v = rnd((1, Lq, 2 * G, D), 1, dt).to(DEV), rnd((1, Lk, 2, D), 2, dt).to(DEV), rnd((1, Lk, 2, D), 3, dt).to(DEV)
             out = K.cross_attention(q, k, v)
             assert out.grad_fn is None and torch.equal(K.cross_attention(q, k.requires_grad_(), v), out)
+
+
+# every form of the forward pass: (Lq, Lk, query heads of a key head, D)
+FORMS = {"token": (1, 300, 1, 64), "split token": (1, 5000, 4, 64), "wide token": (3, 500, 1, 128), "few rows": (20, 700, 1, 64),
+         "wide few rows": (30, 600, 2, 128), "resident keys": (100, 70, 1, 64), "resident wide": (150, 60, 1, 128), "many rows": (200, 300, 1, 64),
+         "many wide rows": (140, 300, 1, 128), "split rows": (70, 3000, 1, 64)}
+INFINITE = ["fp32"]
+
+
+def case(dtype, form, seed=1):
+    Lq, Lk, G, D = FORMS[form]
+    dt = DT[dtype]
+    return rnd((2, Lq, 2 * G, D), seed, dt), rnd((2, Lk, 2, D), seed + 1, dt), rnd((2, Lk, 2, D), seed + 2, dt), rnd((2, Lq, 2 * G, D), seed + 3, dt)
+
+
+@pytest.mark.parametrize("dtype", INFINITE)
+@pytest.mark.parametrize("form", list(FORMS))
+def test_an_infinite_value_is_an_infinity(form, dtype):
+    """every probability is above exp(-20) here and far from underflow, so one infinity among a column's values is the column's sum, two of
+    opposite signs are a NaN, and no other column, head or sequence is touched"""
+    K = ops()
+    Lq, Lk, G, D = FORMS[form]
+    q, k, v, _ = (t.to(DEV) for t in case(dtype, form))
+    scale = D ** -0.5
+    ref = K.cross_attention(q, k, v, None, scale)
+    for sign in (1, -1):
+        for j in (0, 7, Lk - 1):
+            v2 = v.clone()
+            v2[1, j, 1, 9] = sign * math.inf
+            v2[1, Lk // 2, 1, 9] = sign * math.inf
+            out = K.cross_attention(q, k, v2, None, scale)
+            assert bool((out[1, :, G:, 9] == sign * math.inf).all())
+            out[1, :, G:, 9] = ref[1, :, G:, 9]
+            assert torch.equal(out, ref)
+    v2[1, Lk // 3, 1, 9] = math.inf
+    out = K.cross_attention(q, k, v2, None, scale)
+    assert bool(out[1, :, G:, 9].isnan().all())
+    out[1, :, G:, 9] = ref[1, :, G:, 9]
+    assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("dtype", INFINITE)
+@pytest.mark.parametrize("form", list(FORMS))
+def test_an_infinite_output_gradient(form, dtype):
+    """reaches its column of the values' gradient as an infinity, its row and its head's keys as no finite number, and nothing else"""
+    Lq, Lk, G, D = FORMS[form]
+    q, k, v, do = case(dtype, form)
+    clean = run(q, k, v, None, D ** -0.5, do)
+    for sign in (1, -1):
+        do2 = do.clone()
+        do2[1, Lq // 2, -1, 3] = sign * math.inf
+        got = run(q, k, v, None, D ** -0.5, do2)
+        assert bool((got["dv"][1, :, 1, 3] == sign * math.inf).all())
+        assert not bool(torch.isfinite(got["dq"][1, Lq // 2, -1]).any() or torch.isfinite(got["dk"][1, :, 1]).any())
+        got["dv"][1, :, 1, 3] = clean["dv"][1, :, 1, 3]
+        got["dq"][1, Lq // 2, -1] = clean["dq"][1, Lq // 2, -1]
+        got["dk"][1, :, 1] = clean["dk"][1, :, 1]
+        for n, t in got.items():
+            assert torch.equal(t, clean[n]), n
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_the_largest_fp32_keys_are_numbers(form):
+    """keys between bf16's largest (3.3895e38) and fp32's, beside queries of 2^-124: scores of ordinary size"""
+    Lq, Lk, G, D = FORMS[form]
+    q, k, v, do = case("fp32", form)
+    q[..., 5] = torch.where(q[..., 5] > 0, 2.0 ** -124, -2.0 ** -124)
+    k[:, ::3, :, 5] = torch.linspace(3.39e38, torch.finfo(torch.float32).max, len(k[0, ::3]))[None, :, None]
+    do *= 2.0 ** -8                                                              # the queries' gradient in column 5 stays in the type
+    got = run(q, k, v, None, D ** -0.5, do)
+    assert all(bool(torch.isfinite(t).all()) for t in got.values())
+    val, bound = oracle(q, k, v, None, D ** -0.5, do)
+    # the keys' gradients in column 5 are sums of products with 2^-124 and lie below the smallest normal number, on the grid of 2^-149: each
+    # of the roundings of such a sum (six products of every row, the scale, the split sums) is off by half a step of it, 2^-150
+    bound["dk"][..., 5] += (6 * G * Lq + 8) * 2.0 ** -150
+    check(got, val, bound, torch.float32, norms=False)
