@@ -1229,17 +1229,18 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
     const char* const db = (const char*)a.dout + (b * a.d_b + (int64_t)kv * a.G * a.d_h) * T::ES;
     const auto fetch = [&](int r) {
         const int g0 = uniform(r / a.Lq), i0 = r - g0 * a.Lq, here = min(rend - r, a.Lq - i0);      // rows of head g0 from here on
-        if (here >= min(rend - r, C::BR)) {                                // the tile's rows are of one head
+        if (here >= C::BR) {                                               // the tile's rows are of one head
             sq.load(tid, a.D, qb + (i0 * a.q_l + g0 * a.q_h) * T::ES, a.q_l * T::ES, here);
             sd.load(tid, a.D, db + (i0 * a.d_l + g0 * a.d_h) * T::ES, a.d_l * T::ES, here);
         } else {
-            const auto at = [&](int x, const char* base, int64_t sl, int64_t sh) -> const char* {
-                if (r + x >= rend) return nullptr;
-                const int g = (r + x) / a.Lq, i = r + x - g * a.Lq;
+            // Behind the last row: its query again, whose score with an infinite key is no NaN unless that row's own is (zeros would make one),
+            // and an output gradient of zeros; the log-sum of +infinity makes its probabilities 0.
+            const auto at = [&](int x, const char* base, int64_t sl, int64_t sh) {
+                const int g = x / a.Lq, i = x - g * a.Lq;
                 return base + (i * sl + g * sh) * T::ES;
             };
-            sq.gather(tid, a.D, [&](int x) { return at(x, qb, a.q_l, a.q_h); });
-            sd.gather(tid, a.D, [&](int x) { return at(x, db, a.d_l, a.d_h); });
+            sq.gather(tid, a.D, [&](int x) { return at(min(r + x, rend - 1), qb, a.q_l, a.q_h); });
+            sd.gather(tid, a.D, [&](int x) { return r + x < rend ? at(r + x, db, a.d_l, a.d_h) : nullptr; });
         }
         const int x = r + tid % C::BR;
         if (tid < C::BR) st = x < rend ? a.lse[(int64_t)bh * a.R + x] - T::PSHIFT : INFINITY;

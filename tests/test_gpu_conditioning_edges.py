@@ -87,6 +87,31 @@ def test_an_infinite_value_is_an_infinity(form, dtype):
     assert torch.equal(out, ref)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("form", list(FORMS))
+def test_an_infinite_key_takes_no_part_or_all(form, dtype):
+    """a score of -infinity is a key that is not there (its value and key get gradients of 0, and 0 times the infinity is a NaN in the
+    query's gradient, in that column), one of +infinity a NaN row, as the signs of the queries say"""
+    Lq, Lk, G, D = FORMS[form]
+    q, k, v, do = case(dtype, form)
+    q[..., 5] = q[..., 5].abs() + 0.125
+    pad = torch.zeros(2, Lk, dtype=torch.bool)
+    pad[1, 11] = True
+    val, bound = oracle(q, k, v, pad, D ** -0.5, do)
+    k2 = k.clone()
+    k2[1, 11, :, 5] = -math.inf
+    got = run(q, k2, v, None, D ** -0.5, do)
+    assert bool(got["dq"][1, :, :, 5].isnan().all())
+    got["dq"][1, :, :, 5] = val["dq"][1, :, :, 5].to(DEV, DT[dtype])
+    check(got, val, bound, DT[dtype], norms=False)
+    q[1, ::2, :, 5] *= -1
+    out = ops().cross_attention(*(t.to(DEV) for t in (q, k2, v)), None, D ** -0.5)
+    assert bool(out[1, ::2].isnan().all())
+    val, bound = oracle(q, k, v, pad, D ** -0.5, do)
+    out[1, ::2] = val["out"][1, ::2].to(DEV, DT[dtype])
+    check({"out": out}, val, bound, DT[dtype], norms=False)
+
+
 @pytest.mark.parametrize("dtype", INFINITE)
 @pytest.mark.parametrize("form", list(FORMS))
 def test_an_infinite_output_gradient(form, dtype):
