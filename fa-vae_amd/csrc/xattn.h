@@ -81,10 +81,10 @@ template <bool PROB = false>
 __device__ __forceinline__ void split2(float a, float b, unsigned& hi, unsigned& mid, unsigned& lo) {
     constexpr float MOST = 0x1.fep127f;
     const bool ia = !PROB && __builtin_isinf(a), ib = !PROB && __builtin_isinf(b);
-    const float fa = ia ? 0.f : a, fb = ib ? 0.f : b;
-    hi = PROB ? pack2<BF16>(a, b) : pack2<BF16>(__builtin_amdgcn_fmed3f(fa, -MOST, MOST), __builtin_amdgcn_fmed3f(fb, -MOST, MOST));
+    hi = PROB ? pack2<BF16>(a, b)
+              : pack2<BF16>(__builtin_amdgcn_fmed3f(ia ? 0.f : a, -MOST, MOST), __builtin_amdgcn_fmed3f(ib ? 0.f : b, -MOST, MOST));
     const fx2 h = unpack2<BF16>(hi);
-    const float ra = fa - h.x, rb = fb - h.y;                              // a NaN gets here, whatever the median made of it
+    const float ra = ia ? 0.f : a - h.x, rb = ib ? 0.f : b - h.y;          // a NaN gets here, whatever the median made of it
     mid = pack2<BF16>(ra, rb);
     const fx2 m = unpack2<BF16>(mid);
     lo = pack2<BF16>(ia ? a : ra - m.x, ib ? b : rb - m.y);
@@ -240,6 +240,19 @@ template <int TY, int DP, int ROWS, int NT> struct Stage {
 #pragma unroll
             for (int j = 0; j < 4; ++j) r[i][j] = kp ? r[i][j] : 0u;
         }
+    }
+    // some value of this thread's is finite and of 2^120 or more (fp32, bf16)
+    __device__ __forceinline__ bool huge() const {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const unsigned u = r[i][j];
+                any = any || (u & 0x7fffffffu) - 0x7b800000u < 0x04000000u;
+                if constexpr (TY == BF16) any = any || (u << 16 & 0x7fffffffu) - 0x7b800000u < 0x04000000u;
+            }
+        return any;
     }
     __device__ __forceinline__ void store(short* t, int tid) const {
 #pragma unroll
@@ -402,6 +415,21 @@ template <int BK> struct KeyBits {
     }
 };
 
+// The sums of probabilities times values are divided at the end, so they leave 32 bits where values times the number of keys (times 2^LAZY)
+// exceed 3.4e38, although the result does not.  Where a pass over the keys ends with such a sum, it is made once more with probabilities
+// times SMALLER: a power of two, so everything that stayed in range comes out with the same bits.  (fp16 values are below 2^16 and need
+// none of this; infinite and NaN values are passed over twice, too.)
+constexpr float SMALLER = 0x1p-40f;
+template <bool SMALL> __device__ __forceinline__ float prob(float x) { return SMALL ? exp2_f(x) * SMALLER : exp2_f(x); }
+template <int N, typename V> __device__ __forceinline__ bool left_range(const V (&o)[N]) {
+    float z = 0.f;
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(V) / 4); ++i) z = fmaf(o[t][i], 0.f, z);
+    return !(z == 0.f);
+}
+
 // key masks: a tile's scores start at 0 for a key and at -infinity for padding, as the accumulator of their first product
 __device__ __forceinline__ f32x16 start16(const float* bias, int half) {
     f32x16 s;
@@ -488,98 +516,109 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
     load_row<TY, DP>(lane_row<TY>(a, a.q, bh, row0, lane, a.q_b, a.q_l, a.q_h), a.D, lane, qf);
     kend = last_key<C::NT>(pad, k0, kend, tid, red);
     f32x16 o[DP / 32];
-    float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t) o[t] = zero16();
-
+    float m, l, up = 1.f;                                                  // up: what brings l back to its size
     int buf = 0;
-    for (int key = k0; key < kend; key += C::BK) {
-        if (!C::PRE) fetch(key);
-        unsigned long long word[KeyBits<C::BK>::N];
-        const bool all = pb.words(kend - key, word);
-        short* const kt = lds + buf * 2 * C::TILE;
-        short* const vt = kt + C::TILE;
-        float* const bi = bias + buf * C::BK;
-        if (C::BUFS == 1) __syncthreads();
-        if (!all) {
-            const auto keep = [&](int r) { return (bool)((C::BK > 64 && r >= 64 ? word[KeyBits<C::BK>::N - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
-            sk.blank(tid, keep);
-            sv.blank(tid, keep);
-            if (tid < C::BK) bi[tid] = keep(tid) ? 0.f : -INFINITY;
-        }
-        sk.store(kt, tid);
-        sv.store(vt, tid);
-        __syncthreads();
-        if (C::PRE && key + C::BK < kend) fetch(key + C::BK);
-        if (C::BUFS == 2) buf ^= 1;
+    const auto pass = [&](auto smaller) {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) o[t] = zero16();
+        for (int key = k0; key < kend; key += C::BK) {
+            if (!C::PRE) fetch(key);
+            unsigned long long word[KeyBits<C::BK>::N];
+            const bool all = pb.words(kend - key, word);
+            short* const kt = lds + buf * 2 * C::TILE;
+            short* const vt = kt + C::TILE;
+            float* const bi = bias + buf * C::BK;
+            if (C::BUFS == 1) __syncthreads();
+            if (!all) {
+                const auto keep = [&](int r) { return (bool)((C::BK > 64 && r >= 64 ? word[KeyBits<C::BK>::N - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
+                sk.blank(tid, keep);
+                sv.blank(tid, keep);
+                if (tid < C::BK) bi[tid] = keep(tid) ? 0.f : -INFINITY;
+            }
+            sk.store(kt, tid);
+            sv.store(vt, tid);
+            __syncthreads();
+            if (C::PRE && key + C::BK < kend) fetch(key + C::BK);
+            if (C::BUFS == 2) buf ^= 1;
 
-        const int sub0 = KEYW ? w : 0;                                     // this wave's first group of 32 keys
-        if (KEYW && w >= C::NW) continue;
-        f32x16 s[C::KS];
-        if (all) {
+            const int sub0 = KEYW ? w : 0;                                     // this wave's first group of 32 keys
+            if (KEYW && w >= C::NW) continue;
+            f32x16 s[C::KS];
+            if (all) {
 #pragma unroll
-            for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK, true>(kt, 32 * (sub0 + t), qf, bi, lane);
-        } else {
+                for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK, true>(kt, 32 * (sub0 + t), qf, bi, lane);
+            } else {
 #pragma unroll
-            for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK, false>(kt, 32 * (sub0 + t), qf, bi + 32 * (sub0 + t), lane);
-        }
-        constexpr bool AHEAD = !KEYW && TY != F32 && DP <= 64;
-        Frag<T::PL> vf[2 * C::KS];
-        if constexpr (AHEAD) {
+                for (int t = 0; t < C::KS; ++t) s[t] = scores<TY, DP, C::BK, false>(kt, 32 * (sub0 + t), qf, bi + 32 * (sub0 + t), lane);
+            }
+            constexpr bool AHEAD = !KEYW && TY != F32 && DP <= 64;
+            Frag<T::PL> vf[2 * C::KS];
+            if constexpr (AHEAD) {
 #pragma unroll
-            for (int j = 0; j < 2 * C::KS; ++j) vf[j] = col_frag<TY, DP, C::BK>(vt, 16 * j, 0, lane);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        float mx = s[0][0];
+                for (int j = 0; j < 2 * C::KS; ++j) vf[j] = col_frag<TY, DP, C::BK>(vt, 16 * j, 0, lane);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < C::KS; ++t)
+            for (int t = 0; t < C::KS; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-        mx = fmaxf(mx, other_half(mx));
-        if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > LAZY)) {          // some row of this wave outgrew its maximum
-            const float to = fmaxf(m, mx), f = to > m ? exp2_f((m - to) * a.c) : 1.f;
-            l *= f;
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+            mx = fmaxf(mx, other_half(mx));
+            if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > LAZY)) {          // some row of this wave outgrew its maximum
+                const float to = fmaxf(m, mx), f = to > m ? exp2_f((m - to) * a.c) : 1.f;
+                l *= f;
+#pragma unroll
+                for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[t][i] *= f;
+                m = to;
+            }
+            const float sh = T::FSHIFT - (m == -INFINITY ? 0.f : m * a.c);
+            Frag<T::PL> pf[2 * C::KS];
+#pragma unroll
+            for (int t = 0; t < C::KS; ++t) {
+                float p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = prob<decltype(smaller)::value>(fmaf(s[t][i], a.c, sh));
+                    l += p[i];
+                }
+                pf[2 * t] = make_frag<TY, true>(p);
+                pf[2 * t + 1] = make_frag<TY, true>(p + 8);
+                if constexpr (KEYW && TY != F32) {                             // few rows: the matrix pipe has time for what p loses in 16 bits
+                    const Frag<T::PL> r0 = rest_frag<TY>(p, pf[0]), r1 = rest_frag<TY>(p + 8, pf[1]);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) {
+                        o[d] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0, 32 * d, lane), r0, o[d]);
+                        o[d] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16, 32 * d, lane), r1, o[d]);
+                    }
+                }
+            }
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][i] *= f;
-            m = to;
-        }
-        const float sh = T::FSHIFT - (m == -INFINITY ? 0.f : m * a.c);
-        Frag<T::PL> pf[2 * C::KS];
-#pragma unroll
-        for (int t = 0; t < C::KS; ++t) {
-            float p[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                p[i] = exp2_f(fmaf(s[t][i], a.c, sh));
-                l += p[i];
-            }
-            pf[2 * t] = make_frag<TY, true>(p);
-            pf[2 * t + 1] = make_frag<TY, true>(p + 8);
-            if constexpr (KEYW && TY != F32) {                             // few rows: the matrix pipe has time for what p loses in 16 bits
-                const Frag<T::PL> r0 = rest_frag<TY>(p, pf[0]), r1 = rest_frag<TY>(p + 8, pf[1]);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
-                    o[d] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0, 32 * d, lane), r0, o[d]);
-                    o[d] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16, 32 * d, lane), r1, o[d]);
-                }
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-            for (int j = 0; j < 2 * C::KS; ++j) {
-                if constexpr (AHEAD) {
-                    o[t] = mma<TY>(vf[j], pf[j], o[t]);
-                    if (t + 1 < DP / 32) {
-                        vf[j] = col_frag<TY, DP, C::BK>(vt, 16 * j, 32 * (t + 1), lane);
-                        __builtin_amdgcn_sched_barrier(0);
+                for (int j = 0; j < 2 * C::KS; ++j) {
+                    if constexpr (AHEAD) {
+                        o[t] = mma<TY>(vf[j], pf[j], o[t]);
+                        if (t + 1 < DP / 32) {
+                            vf[j] = col_frag<TY, DP, C::BK>(vt, 16 * j, 32 * (t + 1), lane);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    } else {
+                        o[t] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16 * j, 32 * t, lane), pf[j], o[t]);
                     }
-                } else {
-                    o[t] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16 * j, 32 * t, lane), pf[j], o[t]);
                 }
-            }
+        }
+    };
+    pass(std::false_type{});
+    if constexpr (TY != F16) {
+        if (uniform(__syncthreads_or(left_range(o)))) {
+            if (C::PRE) fetch(k0);
+            pass(std::true_type{});
+            up = 1.f / SMALLER;
+        }
     }
 
     const float lt = l + other_half(l);
@@ -609,7 +648,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
                 if (w < C::NW) acc[(w * DP + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3)) * 32 + (lane & 31)] = o[t][i] * inv;
         __syncthreads();
         if (w == 0 && half == 0 && row < a.R) {
-            const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L) - T::FSHIFT);
+            const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L * up) - T::FSHIFT);
             if (a.nsplit > 1) a.part_lse[((int64_t)split * a.B * a.Hkv + bh) * a.R + row] = ls;
             else if (a.lse) a.lse[(int64_t)bh * a.R + row] = L == 0.f ? INFINITY : ls;
         }
@@ -632,7 +671,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         }
     } else {
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
-        const float ls = lt == 0.f ? -INFINITY : m * a.c + (__builtin_amdgcn_logf(lt) - T::FSHIFT);
+        const float ls = lt == 0.f ? -INFINITY : m * a.c + (__builtin_amdgcn_logf(lt * up) - T::FSHIFT);
         const int64_t flat = ((int64_t)split * a.B * a.Hkv + bh) * a.R + row;
         const bool in = row < a.R;
         const OutRows to_row(a, bh, row0);
@@ -705,6 +744,7 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
     const int id = xcd_remap(blockIdx.x, gridDim.x), bh = uniform(id / a.tiles), b = uniform(bh / a.Hkv), kv = bh - b * a.Hkv;
     const int r0 = (id - bh * a.tiles) * a.span, rend = min(a.R, r0 + a.span);  // this workgroup's rows; span is a multiple of 128
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
+    bool huge = false;
     {
         Stage<TY, DP, C::KEYS, C::NT> sk, sv;
         sk.load(tid, a.D, (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES, a.k_l * T::ES, a.Lk);
@@ -717,8 +757,13 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
         sk.store(kt, tid);
         sv.store(vt, tid);
         if (tid < C::KEYS) bias[tid] = keep(tid) ? 0.f : -INFINITY;
+        if constexpr (TY != F16) huge = sv.huge();
     }
-    __syncthreads();
+    // Probabilities are at most 1: fp16 takes them times 2^15.  Their sums with values of 2^120 and more could leave 32 bits before they are
+    // divided: there they are formed times 2^-16 (and their exponents' argument is rounded at 2^-20, which is why not everywhere).
+    float shift = T::PSHIFT;
+    if constexpr (TY == F16) __syncthreads();
+    else if (uniform(__syncthreads_or(huge))) shift = -16.f;
     const int nk = (a.Lk + 31) / 32;                                       // groups of 32 keys; behind the last key: bias -infinity
 
     const auto row_ptr = [&](int rt) { return rt < rend ? lane_row<TY>(a, a.q, bh, rt, lane, a.q_b, a.q_l, a.q_h) : nullptr; };
@@ -740,7 +785,7 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
                 for (int i = 0; i < 16; ++i) m = fmaxf(m, s[t][i]);
             }
         m = fmaxf(m, other_half(m));
-        const float sh = T::PSHIFT - (m == -INFINITY ? 0.f : m * a.c);     // probabilities of at most 1: fp16 takes them times 2^15
+        const float sh = shift - (m == -INFINITY ? 0.f : m * a.c);
         float l = 0.f;
         f32x16 o[DP / 32];
 #pragma unroll
@@ -764,7 +809,7 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
         l += other_half(l);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const OutRows to_row(a, bh, rt);
-        if (half == 0 && in && a.lse) a.lse[(int64_t)bh * a.R + row] = l == 0.f ? INFINITY : m * a.c + (__builtin_amdgcn_logf(l) - T::PSHIFT);
+        if (half == 0 && in && a.lse) a.lse[(int64_t)bh * a.R + row] = l == 0.f ? INFINITY : m * a.c + (__builtin_amdgcn_logf(l) - shift);
         if (TY == F32 || a.o32) {
             float* const to = TY == F32 ? (float*)a.o : a.o32;
             const int64_t at = in ? to_row.at(a, bh, lane & 31) : 0;
@@ -926,61 +971,72 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
     }
     kend = last_key<C::NT>(pad, k0, kend, tid, red);
     fx4 o[DP / 16];
-    float m = -INFINITY, l = 0.f;
+    float m, l, up = 1.f;                                                  // up: what brings l back to its size
+    const auto pass = [&](auto smaller) {
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) o[t] = (fx4){0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < DP / 16; ++t) o[t] = (fx4){0.f, 0.f, 0.f, 0.f};
+        for (int key = k0; key < kend; key += C::BK) {
+            unsigned long long word[KeyBits<C::BK>::N];
+            const bool all = pb.words(kend - key, word);
+            __syncthreads();
+            if (!all) {
+                const auto keep = [&](int r) { return (bool)((r >= 64 ? word[KeyBits<C::BK>::N - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
+                sk.blank(tid, keep);
+                sv.blank(tid, keep);
+                if (tid < C::BK) bias[tid] = keep(tid) ? 0.f : -INFINITY;
+            }
+            sk.store(kt, tid);
+            sv.store(vt, tid);
+            __syncthreads();
+            if (key + C::BK < kend) fetch(key + C::BK);
+            if (w >= C::NW) continue;
 
-    for (int key = k0; key < kend; key += C::BK) {
-        unsigned long long word[KeyBits<C::BK>::N];
-        const bool all = pb.words(kend - key, word);
-        __syncthreads();
-        if (!all) {
-            const auto keep = [&](int r) { return (bool)((r >= 64 ? word[KeyBits<C::BK>::N - 1] >> (r & 63) : word[0] >> (r & 63)) & 1ull); };
-            sk.blank(tid, keep);
-            sv.blank(tid, keep);
-            if (tid < C::BK) bias[tid] = keep(tid) ? 0.f : -INFINITY;
+            fx4 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                s[t] = (fx4){0.f, 0.f, 0.f, 0.f};
+                if (!all) s[t] = *reinterpret_cast<const fx4*>(bias + 32 * w + 16 * t + 4 * quad);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) s[t] = mma16<TY>(row_frag16<TY, DP, C::BK>(kt, 32 * w + 16 * t, d, lane), qf[d], s[t]);
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > LAZY)) {
+                const float to = fmaxf(m, mx), f = to > m ? exp2_f((m - to) * a.c) : 1.f;
+                l *= f;
+#pragma unroll
+                for (int t = 0; t < DP / 16; ++t) o[t] *= f;
+                m = to;
+            }
+            const float sh = T::FSHIFT - (m == -INFINITY ? 0.f : m * a.c);
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                p[i] = prob<decltype(smaller)::value>(fmaf(s[i >> 2][i & 3], a.c, sh));
+                l += p[i];
+            }
+            const Frag<T::PL> pf = make_frag<TY, true>(p);
+            Frag<T::PL> rest;
+            if constexpr (TY != F32) rest = rest_frag<TY>(p, pf);              // the matrix pipe has time for what p loses in 16 bits
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) {
+                const Frag<T::PL> vf = col_frag16<TY, DP, C::BK>(vt, 32 * w, 16 * t, lane);
+                if constexpr (TY != F32) o[t] = mma16<TY>(vf, rest, o[t]);
+                o[t] = mma16<TY>(vf, pf, o[t]);
+            }
         }
-        sk.store(kt, tid);
-        sv.store(vt, tid);
-        __syncthreads();
-        if (key + C::BK < kend) fetch(key + C::BK);
-        if (w >= C::NW) continue;
-
-        fx4 s[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            s[t] = (fx4){0.f, 0.f, 0.f, 0.f};
-            if (!all) s[t] = *reinterpret_cast<const fx4*>(bias + 32 * w + 16 * t + 4 * quad);
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) s[t] = mma16<TY>(row_frag16<TY, DP, C::BK>(kt, 32 * w + 16 * t, d, lane), qf[d], s[t]);
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > LAZY)) {
-            const float to = fmaxf(m, mx), f = to > m ? exp2_f((m - to) * a.c) : 1.f;
-            l *= f;
-#pragma unroll
-            for (int t = 0; t < DP / 16; ++t) o[t] *= f;
-            m = to;
-        }
-        const float sh = T::FSHIFT - (m == -INFINITY ? 0.f : m * a.c);
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[i] = exp2_f(fmaf(s[i >> 2][i & 3], a.c, sh));
-            l += p[i];
-        }
-        const Frag<T::PL> pf = make_frag<TY, true>(p);
-        Frag<T::PL> rest;
-        if constexpr (TY != F32) rest = rest_frag<TY>(p, pf);              // the matrix pipe has time for what p loses in 16 bits
-#pragma unroll
-        for (int t = 0; t < DP / 16; ++t) {
-            const Frag<T::PL> vf = col_frag16<TY, DP, C::BK>(vt, 32 * w, 16 * t, lane);
-            if constexpr (TY != F32) o[t] = mma16<TY>(vf, rest, o[t]);
-            o[t] = mma16<TY>(vf, pf, o[t]);
+    };
+    pass(std::false_type{});
+    if constexpr (TY != F16) {
+        if (uniform(__syncthreads_or(left_range(o)))) {
+            fetch(k0);
+            pass(std::true_type{});
+            up = 1.f / SMALLER;
         }
     }
 
@@ -1010,7 +1066,7 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
             if (w < C::NW) acc[(w * DP + 16 * t + 4 * quad + i) * 16 + row] = o[t][i] * inv;
     __syncthreads();
     if (w == 0 && quad == 0 && row < a.R) {
-        const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L) - T::FSHIFT);
+        const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L * up) - T::FSHIFT);
         if (a.nsplit > 1) a.part_lse[((int64_t)split * heads + bh) * a.R + row] = ls;
         else if (a.lse) a.lse[(int64_t)bh * a.R + row] = L == 0.f ? INFINITY : ls;
     }
@@ -1357,6 +1413,7 @@ __global__ __launch_bounds__(256, (DkvCfg<TY, DP>::WAVES)) void bwd_dkv_kernel(c
 // forward: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  Few splits: a thread owns four columns of a row, bound by the partial
 // results' bytes (two splits of 32768 x 128 columns, 50 MB with the result: 10 us).
 constexpr int MOST_SPLITS = 1024, FEW_SPLITS = 8;
+constexpr float SPARE = 1.f / MOST_SPLITS;               // the weights are formed times this: their sum with values near the largest stays in range
 
 template <int TY>
 __global__ __launch_bounds__(256) void join_few_kernel(const Args a) {
@@ -1380,7 +1437,7 @@ __global__ __launch_bounds__(256) void join_few_kernel(const Args a) {
     const float mr = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int s = 0; s < FEW_SPLITS; ++s) {
-        const float wgt = exp2_f(ls[s] - mr);
+        const float wgt = exp2_f(ls[s] - mr) * SPARE;
         W += wgt;
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = fmaf(wgt, y[s][j], x[j]);
@@ -1389,7 +1446,7 @@ __global__ __launch_bounds__(256) void join_few_kernel(const Args a) {
     const int64_t at = out_at(a, (int)(fr / a.R), (int)(fr % a.R)) + d;
     put4<TY>(a.o, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     if (a.o32) put4<F32>(a.o32, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W);
+    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W * (1.f / SPARE));
 }
 
 // Many splits: a workgroup owns a row, its threads take four columns of every (256 / columns)-th split, so that one latency covers many
@@ -1407,7 +1464,7 @@ __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     const float mr = M == -INFINITY ? 0.f : M;
     float W = 0.f;
-    for (int s = tid; s < a.nsplit; s += 256) W += wgt[s] = exp2_f(wgt[s] - mr);
+    for (int s = tid; s < a.nsplit; s += 256) W += wgt[s] = exp2_f(wgt[s] - mr) * SPARE;
     W = wave_sum(W);
     if (lane == 0) red[4 + w] = W;
     __syncthreads();
@@ -1434,7 +1491,7 @@ __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
     const int64_t at = out_at(a, bh, r) + d;
     put4<TY>(a.o, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     if (a.o32) put4<F32>(a.o32, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W);
+    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W * (1.f / SPARE));
 }
 // backward: out[i] = sum_s part[s][i], s ascending; n a multiple of 4.  8 splits of 0.5 M values: 5 us, about half of it the launch.
 template <int TY>

@@ -147,3 +147,25 @@ def test_the_largest_fp32_keys_are_numbers(form):
     # of the roundings of such a sum (six products of every row, the scale, the split sums) is off by half a step of it, 2^-150
     bound["dk"][..., 5] += (6 * G * Lq + 8) * 2.0 ** -150
     check(got, val, bound, torch.float32, norms=False)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_the_largest_values_are_numbers(form, dtype):
+    """values next to the type's largest (fp32: beyond bf16's, 3.3895e38), as keys beside queries of 2^-124, and as values under no output
+    gradient (whose product with them would leave the type): their sums with undivided probabilities leave 32 bits, the results do not"""
+    Lq, Lk, G, D = FORMS[form]
+    q, k, v, do = case(dtype, form)
+    low, most = 3.39e38 if dtype == "fp32" else 3.3e38, torch.finfo(DT[dtype]).max
+    q[..., 5] = torch.where(q[..., 5] > 0, 2.0 ** -124, -2.0 ** -124)
+    k[:, ::3, :, 5] = torch.linspace(low, most, len(k[0, ::3]))[None, :, None].to(DT[dtype])
+    v[:, 1::5, :, 2] = -torch.linspace(low, most, len(v[0, 1::5]))[None, :, None].to(DT[dtype])
+    do[..., 2] = 0.0
+    do *= 2.0 ** -8                                                              # the queries' gradient in column 5 stays in the type
+    got = run(q, k, v, None, D ** -0.5, do)
+    assert all(bool(torch.isfinite(t).all()) for t in got.values())
+    val, bound = oracle(q, k, v, None, D ** -0.5, do)
+    bound["dk"][..., 5] += (6 * G * Lq + 8) * 2.0 ** -150                        # below the normal numbers, as in the test of the largest keys
+    if dtype == "bf16":
+        bound["dk"][..., 5] += 2.0 ** -134                                       # and rounded to bf16's grid there, 2^-133
+    check(got, val, bound, DT[dtype], norms=False)
