@@ -328,6 +328,20 @@ template <int TY> __device__ __forceinline__ Frag<Ty<TY>::PL> rest_frag(const fl
     return make_frag<TY>(r);
 }
 
+// a 16-bit fragment with zeros for infinities and NaN: the values that the second plane of the probabilities meets.  That plane is 0 or has
+// any sign, where the first one alone gives an infinite value's product.  (All exponent bits plus one step carry into the sign bit.)
+template <int TY, bool CARE> __device__ __forceinline__ Frag<Ty<TY>::PL> finite_frag(const Frag<Ty<TY>::PL>& f) {
+    if constexpr (!CARE) return f;
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    constexpr unsigned EXP = TY == F16 ? 0x7c007c00u : 0x7f807f80u, ONE = TY == F16 ? 0x04000400u : 0x00800080u;
+    ux4 u = __builtin_bit_cast(ux4, f.p[0]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] &= ~__builtin_bit_cast(unsigned, __builtin_bit_cast(s16x2, (u[i] & EXP) + ONE) >> 15);
+    Frag<Ty<TY>::PL> r;
+    r.p[0] = __builtin_bit_cast(s16x8, u);
+    return r;
+}
+
 // four consecutive elements
 template <int TY>
 __device__ __forceinline__ void put4(void* p, int64_t e, float a, float b, float c, float d) {
@@ -415,13 +429,14 @@ template <int BK> struct KeyBits {
     }
 };
 
-// The sums of probabilities times values are divided at the end, so they leave 32 bits where values times the number of keys (times 2^LAZY)
-// exceed 3.4e38, although the result does not.  Where a pass over the keys ends with such a sum, it is made once more with probabilities
-// times SMALLER: a power of two, so everything that stayed in range comes out with the same bits.  (fp16 values are below 2^16 and need
-// none of this; infinite and NaN values are passed over twice, too.)
-constexpr float SMALLER = 0x1p-40f;
-template <bool SMALL> __device__ __forceinline__ float prob(float x) { return SMALL ? exp2_f(x) * SMALLER : exp2_f(x); }
-template <int N, typename V> __device__ __forceinline__ bool left_range(const V (&o)[N]) {
+// A pass over the keys that ends with a sum which is no finite number is made once more, with care:
+//   * the sums of probabilities times values are divided at the end, so they leave 32 bits where values times the number of keys (times
+//     2^LAZY) exceed 3.4e38, although the result does not: probabilities are formed times SMALL (fp16 values are below 2^16 and need none);
+//   * where 16-bit probabilities have a second plane (few rows), it meets zeros for infinities (finite_frag).
+// Both leave the bits of everything that was a number.
+template <int TY> constexpr float SMALL = TY == F16 ? 1.f : 0x1p-40f;
+template <int TY, bool CARE> __device__ __forceinline__ float prob(float x) { return CARE ? exp2_f(x) * SMALL<TY> : exp2_f(x); }
+template <int N, typename V> __device__ __forceinline__ bool not_finite(const V (&o)[N]) {
     float z = 0.f;
 #pragma unroll
     for (int t = 0; t < N; ++t)
@@ -518,7 +533,8 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
     f32x16 o[DP / 32];
     float m, l, up = 1.f;                                                  // up: what brings l back to its size
     int buf = 0;
-    const auto pass = [&](auto smaller) {
+    const auto pass = [&](auto care) {
+        constexpr bool CARE = decltype(care)::value;
         m = -INFINITY;
         l = 0.f;
 #pragma unroll
@@ -582,7 +598,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
                 float p[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    p[i] = prob<decltype(smaller)::value>(fmaf(s[t][i], a.c, sh));
+                    p[i] = prob<TY, CARE>(fmaf(s[t][i], a.c, sh));
                     l += p[i];
                 }
                 pf[2 * t] = make_frag<TY, true>(p);
@@ -591,8 +607,8 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
                     const Frag<T::PL> r0 = rest_frag<TY>(p, pf[0]), r1 = rest_frag<TY>(p + 8, pf[1]);
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) {
-                        o[d] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0, 32 * d, lane), r0, o[d]);
-                        o[d] = mma<TY>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16, 32 * d, lane), r1, o[d]);
+                        o[d] = mma<TY>(finite_frag<TY, CARE>(col_frag<TY, DP, C::BK>(vt, 32 * sub0, 32 * d, lane)), r0, o[d]);
+                        o[d] = mma<TY>(finite_frag<TY, CARE>(col_frag<TY, DP, C::BK>(vt, 32 * sub0 + 16, 32 * d, lane)), r1, o[d]);
                     }
                 }
             }
@@ -613,11 +629,11 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         }
     };
     pass(std::false_type{});
-    if constexpr (TY != F16) {
-        if (uniform(__syncthreads_or(left_range(o)))) {
+    if constexpr (TY != F16 || KEYW) {
+        if (uniform(__syncthreads_or(not_finite(o)))) {
             if (C::PRE) fetch(k0);
             pass(std::true_type{});
-            up = 1.f / SMALLER;
+            up = 1.f / SMALL<TY>;
         }
     }
 
@@ -972,7 +988,8 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
     kend = last_key<C::NT>(pad, k0, kend, tid, red);
     fx4 o[DP / 16];
     float m, l, up = 1.f;                                                  // up: what brings l back to its size
-    const auto pass = [&](auto smaller) {
+    const auto pass = [&](auto care) {
+        constexpr bool CARE = decltype(care)::value;
         m = -INFINITY;
         l = 0.f;
 #pragma unroll
@@ -1017,7 +1034,7 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                p[i] = prob<decltype(smaller)::value>(fmaf(s[i >> 2][i & 3], a.c, sh));
+                p[i] = prob<TY, CARE>(fmaf(s[i >> 2][i & 3], a.c, sh));
                 l += p[i];
             }
             const Frag<T::PL> pf = make_frag<TY, true>(p);
@@ -1026,18 +1043,16 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
 #pragma unroll
             for (int t = 0; t < DP / 16; ++t) {
                 const Frag<T::PL> vf = col_frag16<TY, DP, C::BK>(vt, 32 * w, 16 * t, lane);
-                if constexpr (TY != F32) o[t] = mma16<TY>(vf, rest, o[t]);
+                if constexpr (TY != F32) o[t] = mma16<TY>(finite_frag<TY, CARE>(vf), rest, o[t]);
                 o[t] = mma16<TY>(vf, pf, o[t]);
             }
         }
     };
     pass(std::false_type{});
-    if constexpr (TY != F16) {
-        if (uniform(__syncthreads_or(left_range(o)))) {
-            fetch(k0);
-            pass(std::true_type{});
-            up = 1.f / SMALLER;
-        }
+    if (uniform(__syncthreads_or(not_finite(o)))) {
+        fetch(k0);
+        pass(std::true_type{});
+        up = 1.f / SMALL<TY>;
     }
 
     float lt = l + __shfl_xor(l, 16, 64);

@@ -1984,6 +1984,8 @@ def cross_attention(q, k, v, key_padding_mask=None, scale=None):
     under 16 MiB.
     key_padding_mask: bool (B, Lk), True = this key is padding (nn.MultiheadAttention's meaning); a row that is left without keys gives
     zeros, and whatever padded rows of k and v hold reaches no result.  scale: 1 / sqrt(D) unless given, positive.
+    Infinities and NaN elsewhere do what the formula makes of them, in every form alike; a probability of 0 (underflow) makes a NaN of an
+    infinite value.
     Lq = 1 (a decoding step) and long keys run the same call: the keys are split over the chip.  Differentiable in q, k, v, once and
     backward: forward-mode tangents raise, as second derivatives do."""
     _require_float_gpu("cross_attention", q, k, v)
