@@ -55,10 +55,13 @@ template <int TY> struct Ty {
     static constexpr int PL = TY == F32 ? 3 : 1;         // planes of an operand
     static constexpr int ES = TY == F32 ? 4 : 2;         // bytes of an element
     static constexpr int EPC = 16 / ES;                  // elements of a 16-byte chunk
+    // Forward, the running maximum follows only when a row's scores exceed it by 2^LAZY: p <= 2^LAZY, few rescalings.
     // fp16 keeps 5 exponent bits.  Backward, probabilities (<= 1) are formed times 2^15, so that one of 2^-29 is still a normal number;
-    // forward they may exceed 1 by 2^LAZY (fwd_kernel) and are formed times 2^7.
+    // forward they are formed times 2^13, so that one of 2^-27 of the row's largest is, and below that each is off by up to 2^-38 of the
+    // largest.  (2^8 and 2^7 left 2^-21, and a row whose largest probability meets a value near 0 lost up to four bits of its result.)
     static constexpr float PSHIFT = TY == F16 ? 15.f : 0.f;
-    static constexpr float FSHIFT = TY == F16 ? 7.f : 0.f;
+    static constexpr float LAZY = TY == F16 ? 2.f : 8.f;
+    static constexpr float FSHIFT = TY == F16 ? 15.f - LAZY : 0.f;
 };
 
 template <int PL> struct Frag { s16x8 p[PL]; };
@@ -478,8 +481,6 @@ __device__ __forceinline__ f32x16 scores(const short* t, int row0, const Frag<Ty
 // 64 rows a wave took the same time, two groups with interleaved exponentials 10 % more, four waves (32 keys at a time) 6 %, the next
 // tile's stores between the products 15 %, sums by products with ones 4 %.
 // -------------------------------------------------------------------------------------------------------------------------------------
-constexpr float LAZY = 8.f;      // the running maximum follows only when a row's scores exceed it by 2^8: p <= 2^8, few rescalings
-
 template <int TY, int DP, bool KEYW> struct FwdCfg {
     static constexpr int NT = 256;
     static constexpr int NW = KEYW && TY == F32 && DP > 64 ? 2 : 4;        // waves that compute: the planes of 128 keys of 96, 128 fp32 columns
@@ -582,7 +583,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
 #pragma unroll
                 for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
             mx = fmaxf(mx, other_half(mx));
-            if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > LAZY)) {          // some row of this wave outgrew its maximum
+            if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > T::LAZY)) {       // some row of this wave outgrew its maximum
                 const float to = fmaxf(m, mx), f = to > m ? exp2_f((m - to) * a.c) : 1.f;
                 l *= f;
 #pragma unroll
@@ -1023,7 +1024,7 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > LAZY)) {
+            if (__builtin_amdgcn_ballot_w64((mx - m) * a.c > T::LAZY)) {
                 const float to = fmaxf(m, mx), f = to > m ? exp2_f((m - to) * a.c) : 1.f;
                 l *= f;
 #pragma unroll

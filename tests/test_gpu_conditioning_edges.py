@@ -168,3 +168,20 @@ def test_the_largest_values_are_numbers(form, dtype):
     if dtype == "bf16":
         bound["dk"][..., 5] += 2.0 ** -134                                       # and rounded to bf16's grid there, 2^-133
     check(got, val, bound, DT[dtype], norms=False)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("gap", [21.5, 24.3, 26.7])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_small_probabilities_keep_their_bits(form, gap, dtype):
+    """a key that takes almost everything and whose value is 0, and all others alike, 2^gap below it: nothing averages the rounding of their
+    probabilities, which is that of a normal number of the type"""
+    Lq, Lk, G, D = FORMS[form]
+    dt = DT[dtype]
+    q, k, v, do = case(dtype, form)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[..., 1:] = 0.0
+    k[:, 1, :, 0] = gap * math.log(2.0)
+    v = (v.abs() * 1024 + 512).to(dt)                                            # results that are normal numbers
+    v[:, 1] = 0.0
+    check(run(q, k, v, None, 0.125, do), *oracle(q, k, v, None, 0.125, do), dt, norms=False)
