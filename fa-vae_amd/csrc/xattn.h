@@ -761,13 +761,14 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
     const int id = xcd_remap(blockIdx.x, gridDim.x), bh = uniform(id / a.tiles), b = uniform(bh / a.Hkv), kv = bh - b * a.Hkv;
     const int r0 = (id - bh * a.tiles) * a.span, rend = min(a.R, r0 + a.span);  // this workgroup's rows; span is a multiple of 128
     const uint8_t* const pad = a.pad ? a.pad + b * a.pad_b : nullptr;
-    bool huge = false;
+    bool huge = false, keys;                                               // keys: there is one that is not padding
     {
         Stage<TY, DP, C::KEYS, C::NT> sk, sv;
         sk.load(tid, a.D, (const char*)a.k + (b * a.k_b + kv * a.k_h) * T::ES, a.k_l * T::ES, a.Lk);
         sv.load(tid, a.D, (const char*)a.v + (b * a.v_b + kv * a.v_h) * T::ES, a.v_l * T::ES, a.Lk);
         const bool k0 = lane < a.Lk && !(pad && pad[lane]), k1 = 64 + lane < a.Lk && !(pad && pad[64 + lane]);
         const unsigned long long w0 = __builtin_amdgcn_ballot_w64(k0), w1 = __builtin_amdgcn_ballot_w64(k1);
+        keys = (w0 | w1) != 0;
         const auto keep = [&](int r) { return (bool)((r >= 64 ? w1 >> (r & 63) : w0 >> r) & 1ull); };
         sk.blank(tid, keep);
         sv.blank(tid, keep);
@@ -781,7 +782,8 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
     float shift = T::PSHIFT;
     if constexpr (TY == F16) __syncthreads();
     else if (uniform(__syncthreads_or(huge))) shift = -16.f;
-    const int nk = (a.Lk + 31) / 32;                                       // groups of 32 keys; behind the last key: bias -infinity
+    // groups of 32 keys; behind the last key: bias -infinity.  Without keys there is no group: a query of NaN makes NaN scores of padding, too
+    const int nk = keys ? (a.Lk + 31) / 32 : 0;
 
     const auto row_ptr = [&](int rt) { return rt < rend ? lane_row<TY>(a, a.q, bh, rt, lane, a.q_b, a.q_l, a.q_h) : nullptr; };
     Frag<T::PL> qf[DP / 16];

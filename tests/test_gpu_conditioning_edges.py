@@ -185,3 +185,21 @@ def test_small_probabilities_keep_their_bits(form, gap, dtype):
     v = (v.abs() * 1024 + 512).to(dt)                                            # results that are normal numbers
     v[:, 1] = 0.0
     check(run(q, k, v, None, 0.125, do), *oracle(q, k, v, None, 0.125, do), dt, norms=False)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("form", list(FORMS))
+def test_sequences_without_keys_give_zeros_whatever_their_queries_hold(form, dtype):
+    """and gradients of zeros; a sequence that has keys is not touched"""
+    Lq, Lk, G, D = FORMS[form]
+    q, k, v, do = case(dtype, form)
+    pad = torch.zeros(2, Lk, dtype=torch.bool)
+    pad[0] = True
+    clean = run(q, k, v, pad, D ** -0.5, do)
+    q[0, :, ::2] = math.nan
+    q[0, :, 1::2, 3] = -math.inf
+    k[0, ::2], v[0, 1::2] = math.inf, math.nan
+    got = run(q, k, v, pad, D ** -0.5, do)
+    for n, t in got.items():
+        assert not t[0].any() and not t[0].isnan().any(), n
+        assert torch.equal(t, clean[n]), n
