@@ -435,10 +435,20 @@ template <int BK> struct KeyBits {
 // A pass over the keys that ends with a sum which is no finite number is made once more, with care:
 //   * the sums of probabilities times values are divided at the end, so they leave 32 bits where values times the number of keys (times
 //     2^LAZY) exceed 3.4e38, although the result does not: probabilities are formed times SMALL (fp16 values are below 2^16 and need none);
-//   * where 16-bit probabilities have a second plane (few rows), it meets zeros for infinities (finite_frag).
-// Both leave the bits of everything that was a number.
+//   * where 16-bit probabilities have a second plane (few rows), it meets zeros for infinities (finite_frag);
+//   * c s - c m is one multiply-add with a rounded c m, half a step of which is a factor of 2^8 for c m = 2^33 (and of fp16's range for 2^26):
+//     rows of such maxima take c (s - m) (Ref).  Then the sum of a row's probabilities may be 0, too, although it has keys.
+// All leave the bits of everything that was a number.
 template <int TY> constexpr float SMALL = TY == F16 ? 1.f : 0x1p-40f;
 template <int TY, bool CARE> __device__ __forceinline__ float prob(float x) { return CARE ? exp2_f(x) * SMALL<TY> : exp2_f(x); }
+// the exponent of a row's probabilities is c (s - r) + sh
+struct Ref {
+    float r, sh;
+    __device__ __forceinline__ Ref(float m, float c, float shift, bool care) {
+        r = care && fabsf(m * c) > 0x1p20f && fabsf(m) < INFINITY ? m : 0.f;
+        sh = shift - (m == -INFINITY || r != 0.f ? 0.f : m * c);
+    }
+};
 template <int N, typename V> __device__ __forceinline__ bool not_finite(const V (&o)[N]) {
     float z = 0.f;
 #pragma unroll
@@ -592,14 +602,14 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
                     for (int i = 0; i < 16; ++i) o[t][i] *= f;
                 m = to;
             }
-            const float sh = T::FSHIFT - (m == -INFINITY ? 0.f : m * a.c);
+            const Ref ref(m, a.c, T::FSHIFT, CARE);
             Frag<T::PL> pf[2 * C::KS];
 #pragma unroll
             for (int t = 0; t < C::KS; ++t) {
                 float p[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    p[i] = prob<TY, CARE>(fmaf(s[t][i], a.c, sh));
+                    p[i] = prob<TY, CARE>(fmaf(CARE ? s[t][i] - ref.r : s[t][i], a.c, ref.sh));
                     l += p[i];
                 }
                 pf[2 * t] = make_frag<TY, true>(p);
@@ -630,15 +640,13 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         }
     };
     pass(std::false_type{});
-    if constexpr (TY != F16 || KEYW) {
-        if (uniform(__syncthreads_or(not_finite(o)))) {
-            if (C::PRE) fetch(k0);
-            pass(std::true_type{});
-            up = 1.f / SMALL<TY>;
-        }
+    float lt = l + other_half(l);
+    if (uniform(__syncthreads_or(not_finite(o) || (lt == 0.f && m > -INFINITY)))) {
+        if (C::PRE) fetch(k0);
+        pass(std::true_type{});
+        up = 1.f / SMALL<TY>;
+        lt = l + other_half(l);
     }
-
-    const float lt = l + other_half(l);
     if constexpr (KEYW) {
         // join the waves: row statistics first, then each wave's scaled accumulators through LDS
         if (half == 0 && w < C::NW) {
@@ -804,7 +812,13 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
                 for (int i = 0; i < 16; ++i) m = fmaxf(m, s[t][i]);
             }
         m = fmaxf(m, other_half(m));
-        const float sh = shift - (m == -INFINITY ? 0.f : m * a.c);
+        const Ref ref(m, a.c, shift, true);
+        if (__builtin_amdgcn_ballot_w64(ref.r != 0.f)) {
+#pragma unroll
+            for (int t = 0; t < C::KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] -= ref.r;
+        }
         float l = 0.f;
         f32x16 o[DP / 32];
 #pragma unroll
@@ -815,7 +829,7 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
                 float p[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    p[i] = exp2_f(fmaf(s[t][i], a.c, sh));
+                    p[i] = exp2_f(fmaf(s[t][i], a.c, ref.sh));
                     l += p[i];
                 }
                 const Frag<T::PL> p0 = make_frag<TY, true>(p), p1 = make_frag<TY, true>(p + 8);
@@ -1033,11 +1047,11 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
                 for (int t = 0; t < DP / 16; ++t) o[t] *= f;
                 m = to;
             }
-            const float sh = T::FSHIFT - (m == -INFINITY ? 0.f : m * a.c);
+            const Ref ref(m, a.c, T::FSHIFT, CARE);
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                p[i] = prob<TY, CARE>(fmaf(s[i >> 2][i & 3], a.c, sh));
+                p[i] = prob<TY, CARE>(fmaf(CARE ? s[i >> 2][i & 3] - ref.r : s[i >> 2][i & 3], a.c, ref.sh));
                 l += p[i];
             }
             const Frag<T::PL> pf = make_frag<TY, true>(p);
@@ -1052,14 +1066,17 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
         }
     };
     pass(std::false_type{});
-    if (uniform(__syncthreads_or(not_finite(o)))) {
+    const auto total = [](float x) {
+        x += __shfl_xor(x, 16, 64);
+        return x + __shfl_xor(x, 32, 64);
+    };
+    float lt = total(l);
+    if (uniform(__syncthreads_or(not_finite(o) || (lt == 0.f && m > -INFINITY)))) {
         fetch(k0);
         pass(std::true_type{});
         up = 1.f / SMALL<TY>;
+        lt = total(l);
     }
-
-    float lt = l + __shfl_xor(l, 16, 64);
-    lt += __shfl_xor(lt, 32, 64);
     if (quad == 0 && w < C::NW) {
         stat[w * 16 + row] = m;
         stat[(C::NW + w) * 16 + row] = lt;

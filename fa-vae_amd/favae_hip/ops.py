@@ -1986,6 +1986,8 @@ def cross_attention(q, k, v, key_padding_mask=None, scale=None):
     zeros, and whatever padded rows of k and v hold reaches no result.  scale: 1 / sqrt(D) unless given, positive.
     Infinities and NaN elsewhere do what the formula makes of them, in every form alike; a probability of 0 (underflow) makes a NaN of an
     infinite value.
+    Scores may be of any finite size.  The backward pass forms the probabilities again from 32-bit log-sums, half a step of which is a
+    relative error of |score| / 2^24: scores of 10^4 and more cost gradients their precision, scores above 10^9 their meaning.
     Lq = 1 (a decoding step) and long keys run the same call: the keys are split over the chip.  Differentiable in q, k, v, once and
     backward: forward-mode tangents raise, as second derivatives do."""
     _require_float_gpu("cross_attention", q, k, v)

@@ -203,3 +203,24 @@ def test_sequences_without_keys_give_zeros_whatever_their_queries_hold(form, dty
     for n, t in got.items():
         assert not t[0].any() and not t[0].isnan().any(), n
         assert torch.equal(t, clean[n]), n
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("form", list(FORMS))
+def test_scores_of_any_finite_size(form, dtype):
+    """scores of 1e8 (fp16) and 1e12, whose spacing in 32 bits is more than a softmax can resolve: a row is its largest score's value where
+    the next one is out of reach of the scores' own rounding, (D + 8) 2^-24 of the products' magnitudes, and an average of values elsewhere"""
+    Lq, Lk, G, D = FORMS[form]
+    dt = DT[dtype]
+    q, k, v, _ = case(dtype, form)
+    gain = 1e4 if dtype == "fp16" else 1e6
+    q, k = (q.double() * gain).to(dt), (k.double() * gain).to(dt)
+    out = ops().cross_attention(*(t.to(DEV) for t in (q, k, v)), None, 0.125).cpu().double()
+    qh, kh, vh = q.double().transpose(1, 2), *(t.double().repeat_interleave(G, 2).transpose(1, 2) for t in (k, v))
+    s, mag = 0.125 * qh @ kh.transpose(2, 3), 0.125 * qh.abs() @ kh.abs().transpose(2, 3)
+    top = s.topk(2, 3)
+    clear = top.values[..., 0] - top.values[..., 1] > 2 * (D + 8) * 2.0 ** -24 * mag.amax(3) + 1000
+    best = torch.gather(vh, 2, top.indices[..., :1].expand(-1, -1, -1, D)).transpose(1, 2)
+    assert float(clear.double().mean()) > 0.9 and bool(torch.isfinite(out).all())
+    assert torch.equal(out[clear.transpose(1, 2)], best[clear.transpose(1, 2)])
+    assert bool((out.abs() <= vh.abs().amax(2)[:, None] * (1 + 2 * half_step(dt))).all())
