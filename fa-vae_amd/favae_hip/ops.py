@@ -1876,6 +1876,13 @@ def _require_float_gpu(what, *tensors):
         raise RuntimeError("%s: tensors differ in device or type (%s %s, %s %s)" % (what, t0.device, t0.dtype, t.device, t.dtype))
 
 
+def _number(what, scale):
+    """scale as a float.  A tensor that requires a gradient would get none, without a word"""
+    if isinstance(scale, torch.Tensor) and scale.requires_grad:
+        raise ValueError("%s: scale is a number and gets no gradient (multiply the input by a learnt scale instead)" % what)
+    return float(scale)
+
+
 def _on_device(fn, device, *args):
     """fn(*args) with `device` current: the stream a call goes to is the current one of the tensors' device"""
     if device.index == torch.cuda.current_device():
@@ -1999,7 +2006,7 @@ def cross_attention(q, k, v, key_padding_mask=None, scale=None):
         raise ValueError("cross_attention: %d query heads do not share %d key / value heads evenly" % (H, Hkv))
     if D % 8 or not 8 <= D <= 128:
         raise ValueError("cross_attention: a head has a multiple of 8 columns, 8 to 128 (got %d)" % D)
-    scale = D ** -0.5 if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else _number("cross_attention", scale)
     if not 0.0 < scale < math.inf:
         raise ValueError("cross_attention: scale has to be positive and finite (got %r)" % scale)
     if key_padding_mask is not None:
@@ -2090,7 +2097,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
         raise ValueError("embedding: weight is (V, C), got %s" % (tuple(weight.shape),))
     ids = _check_ids("embedding", ids, weight.device)
     padding = _check_padding_idx("embedding", padding_idx, weight.shape[0])
-    scale = float(scale)
+    scale = _number("embedding", scale)
     if weight.stride(1) != 1 and weight.shape[1] > 1:
         weight = weight.contiguous()
     return EmbeddingFn.apply(weight, ids, scale, padding)
@@ -2108,7 +2115,7 @@ def embedding_grad(dout, ids, rows, scale=1.0, padding_idx=None):
                          % (tuple(dout.shape), tuple(ids.shape), rows))
     ids = _check_ids("embedding_grad", ids, dout.device)
     padding = _check_padding_idx("embedding_grad", padding_idx, rows)
-    return EmbeddingGradFn.apply(dout, ids, rows, float(scale), padding)
+    return EmbeddingGradFn.apply(dout, ids, rows, _number("embedding_grad", scale), padding)
 
 
 # ---------------------------------------------------------------------------------------------------------------

@@ -126,3 +126,15 @@ def test_nothing_is_kept_where_no_gradient_can_be_asked_for(launches, monkeypatc
     with torch.inference_mode():
         K.cross_attention(q, k, v)
     assert out.grad_fn is not None and seen == [False, True, False, False]
+
+
+def test_a_learnt_scale_is_refused(launches):
+    """it would get no gradient; one that needs none is a number like any other"""
+    q, k, v = tensors()
+    ids, w, g = torch.tensor([0, 3, 1]), torch.randn(4, 8), torch.randn(3, 8)
+    learnt = torch.tensor(0.5, requires_grad=True)
+    for f in (lambda s: K.cross_attention(q, k, v, None, s), lambda s: K.embedding(ids, w, s), lambda s: K.embedding_grad(g, ids, 4, s)):
+        with pytest.raises(ValueError, match="no gradient"):
+            f(learnt)
+        f(learnt.detach())
+        f(0.5)
