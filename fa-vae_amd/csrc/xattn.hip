@@ -76,10 +76,12 @@ Plan plan_dkv(const favae_xattn_desc* d) {
     return p;
 }
 
+float args_c(const favae_xattn_desc* d) { return (float)((double)d->scale * 1.4426950408889634); }      // scale in powers of two
+
 // sizes and strides the kernels can take; the byte range of an element type's strides is the caller's memory
 bool ok_desc(const favae_xattn_desc* d) {
     if (!d || d->B < 1 || d->Lq < 1 || d->Lk < 1 || d->H < 1 || d->Hkv < 1 || d->H % d->Hkv || d->D < 8 || d->D > 128 || d->D % 8) return false;
-    if (d->dtype < F32 || d->dtype > F16 || !(d->scale > 0.f) || !(d->scale < INFINITY)) return false;
+    if (d->dtype < F32 || d->dtype > F16 || !(d->scale > 0.f) || !(args_c(d) < INFINITY)) return false;
     const int64_t R = (int64_t)d->H / d->Hkv * d->Lq, heads = (int64_t)d->B * d->Hkv;
     if (R > (1 << 30) || d->Lk > (1 << 30) || heads > (1 << 24)) return false;
     if (((R + 31) / 32 > (d->Lk + 127) / 128 ? (R + 31) / 32 : (d->Lk + 127) / 128) * heads >= (1 << 24)) return false;   // 2^32 threads a launch
@@ -104,7 +106,7 @@ Args args_of(const favae_xattn_desc* d, const void* q, const void* k, const void
     a.B = d->B; a.Lq = d->Lq; a.Lk = d->Lk; a.H = d->H; a.Hkv = d->Hkv; a.G = d->H / d->Hkv; a.D = d->D;
     a.R = a.G * a.Lq;
     a.scale = d->scale;
-    a.c = (float)((double)d->scale * 1.4426950408889634);
+    a.c = args_c(d);
     return a;
 }
 void use(Args& a, const Plan& p) { a.tiles = p.tiles; a.nsplit = p.nsplit; a.span = p.span; }

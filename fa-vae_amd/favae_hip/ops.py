@@ -1990,7 +1990,7 @@ def cross_attention(q, k, v, key_padding_mask=None, scale=None):
     tensors are read in place where their rows are contiguous and 16-byte aligned, other layouts are copied first); H * D values
     under 16 MiB.
     key_padding_mask: bool (B, Lk), True = this key is padding (nn.MultiheadAttention's meaning); a row that is left without keys gives
-    zeros, and whatever padded rows of k and v hold reaches no result.  scale: 1 / sqrt(D) unless given, positive.
+    zeros, and whatever padded rows of k and v hold reaches no result.  scale: 1 / sqrt(D) unless given, positive and below 2.3e38.
     Infinities and NaN elsewhere do what the formula makes of them, in every form alike; a probability of 0 (underflow) makes a NaN of an
     infinite value.
     Scores may be of any finite size.  The backward pass forms the probabilities again from 32-bit log-sums, half a step of which is a

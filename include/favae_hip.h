@@ -517,7 +517,7 @@ int favae_gn_act_bwd_tiles(const float* da, const float* x, const float* gamma, 
  *   o = softmax over the keys of scale * <q, k> that are not padding, times v; a row without keys gives zeros, and zero gradients.
  * Strides are in elements, for q, k, v (batch, length, head; columns contiguous, each stride a multiple of 16 bytes, 0 allowed but for the
  * length: that one is at least D and below 2^24 bytes); o, dout and the gradients are dense (H * D elements below 2^24 bytes too).
- * D % 8 == 0, 8 <= D <= 128, scale > 0.  key_padding_mask: NULL, or B rows of Lk bytes pad_sb bytes apart, nonzero = this key is padding:
+ * D % 8 == 0, 8 <= D <= 128, 0 < scale < 2.3e38.  key_padding_mask: NULL, or B rows of Lk bytes pad_sb bytes apart, nonzero = this key is padding:
  * what its rows of k and v hold (infinities, NaN) reaches no result and its gradients are zeros.
  * Every data pointer is 16-byte aligned.  Results do not depend on anything but the arguments (no atomics on floats). */
 typedef struct {

@@ -135,3 +135,13 @@ def test_rows_of_very_many_heads_are_refused():
         at, under = (desc(B=1, Lq=1, Lk=1, H=h, Hkv=8, D=64, dtype=dtype) for h in (heads, heads - 8))
         assert lib.favae_xattn_bwd_workspace(byref(at)) == 0 and lib.favae_xattn_bwd_workspace(byref(under)) > 0
         assert lib.favae_xattn_fwd(byref(at), 1 << 12, 1 << 12, 1 << 12, None, 1 << 12, None, None, None, 0, None) == 3
+
+
+def test_scales_that_leave_32_bits_in_powers_of_two_are_refused():
+    """scores are taken times scale / ln 2"""
+    lib = favae_hip.load()
+    for scale, ok in ((2.3e38, True), (2.4e38, False), (3.4e38, False)):
+        d = desc(scale=scale)
+        assert (lib.favae_xattn_bwd_workspace(byref(d)) > 0) == ok
+        if not ok:
+            assert lib.favae_xattn_fwd(byref(d), 1 << 12, 1 << 12, 1 << 12, None, 1 << 12, None, None, None, 0, None) == 3
