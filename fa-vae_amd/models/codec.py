@@ -15,6 +15,7 @@ Reference map (file:line in the reference repo):
 """
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from favae_hip import ACT_NONE, ACT_SILU
 from favae_hip import ops as K
@@ -129,7 +130,8 @@ class CrossAttnBlock(nn.Module):
     """Image tokens attend to the states of another sequence: x + proj(attention(q(GroupNorm(x)), kv(states))).  The reference has no such
     block (its codec attends within the image); it is laid out like AttnBlock and TransEncoderBlock (GroupNorm(32), 8 heads): the
     projections are 1x1 convs, the two halves of `kv` are read in place.  states (B, L, ctx_c) of any length; padding (B, L) bool, True =
-    not a token (nn.MultiheadAttention's key_padding_mask).  An image whose states are all padding passes through with proj's bias."""
+    not a token (nn.MultiheadAttention's key_padding_mask).  An image whose states are all padding, or none, passes through with proj's
+    bias."""
 
     def __init__(self, in_c, ctx_c, num_heads=8):
         super().__init__()
@@ -145,8 +147,12 @@ class CrossAttnBlock(nn.Module):
     def forward(self, x, states, padding=None):
         q, xa = K.fused_conv(x, self.q.weight, self.q.bias, self.norm.weight, self.norm.bias, None, self._cfg_in, True)
         B, C, H, W = q.shape
-        kv = K.fused_conv(states.transpose(1, 2).unsqueeze(2), self.kv.weight, self.kv.bias, cfg=_C1)      # (B, 2C, 1, L)
-        k, v = kv.permute(0, 2, 3, 1).reshape(B, -1, 2, self.num_heads, C // self.num_heads).unbind(2)
+        L = states.shape[1]
+        if L:
+            kv = K.fused_conv(states.transpose(1, 2).unsqueeze(2), self.kv.weight, self.kv.bias, cfg=_C1).permute(0, 2, 3, 1)  # (B, 1, L, 2C)
+        else:                                                     # a conv has no form without pixels; nothing is computed here
+            kv = F.linear(states, self.kv.weight, self.kv.bias)
+        k, v = kv.reshape(B, L, 2, self.num_heads, C // self.num_heads).unbind(2)
         o = K.cross_attention(q.permute(0, 2, 3, 1).reshape(B, H * W, self.num_heads, -1), k, v, padding)
         return K.fused_conv(o.view(B, H, W, C).permute(0, 3, 1, 2), self.proj.weight, self.proj.bias, resid=xa, cfg=_C1)
 

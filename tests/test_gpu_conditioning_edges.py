@@ -224,3 +224,24 @@ def test_scores_of_any_finite_size(form, dtype):
     assert float(clear.double().mean()) > 0.9 and bool(torch.isfinite(out).all())
     assert torch.equal(out[clear.transpose(1, 2)], best[clear.transpose(1, 2)])
     assert bool((out.abs() <= vh.abs().amax(2)[:, None] * (1 + 2 * half_step(dt))).all())
+
+
+def test_block_over_no_states_is_the_identity_and_its_bias():
+    """a prompt of length 0, as one that is all padding: the same result, and gradients of zeros for what nothing depends on"""
+    from models.codec import CrossAttnBlock
+    torch.manual_seed(3)
+    blk = CrossAttnBlock(64, 48, num_heads=4).to(DEV)
+    x, do = rnd((3, 64, 8, 8), 2, torch.float32).to(DEV).requires_grad_(), rnd((3, 64, 8, 8), 4, torch.float32).to(DEV)
+    results = []
+    for states, pad in ((torch.zeros(3, 0, 48, device=DEV), torch.zeros(3, 0, dtype=torch.bool, device=DEV)), (torch.zeros(3, 0, 48, device=DEV), None),
+                        (torch.ones(3, 5, 48, device=DEV), torch.ones(3, 5, dtype=torch.bool, device=DEV))):
+        states.requires_grad_()
+        y = blk(x, states, pad)
+        leaves = [x, states] + list(blk.parameters())
+        results.append([y] + list(torch.autograd.grad(y, leaves, do)))
+        names = ["y", "x", "states"] + [n for n, _ in blk.named_parameters()]
+        assert torch.equal(y, x + blk.proj.bias[:, None, None]) and torch.equal(results[-1][1], do)
+        for n, t in zip(names, results[-1]):
+            assert bool(torch.isfinite(t).all()) and (n in ("y", "x", "proj.bias") or not t.any()), n
+    for n, a, b in zip(names, results[0], results[2]):
+        assert n == "states" or torch.equal(a, b), n
