@@ -536,7 +536,6 @@ template <int TY, bool VEC>
 int go_sums(const uint2* sorted, const unsigned* valid, const void* dout, void* dw, float* part, int64_t T, int C, const Plan& p, float scale, hipStream_t s) {
     const int per = 64 * Piece<TY, VEC>::N, nseg = (C + per - 1) / per;
     const int64_t blocks = (p.chunks * nseg + 3) / 4;
-    if (blocks >= 1 << 24) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);
     FAVAE_KLAUNCH((embed_sum_kernel<TY, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, sorted, valid, dout, dw, part, T, C, p.chunk, nseg, scale);
     FAVAE_CHECK_LAUNCH();
     if (p.chunks > 1) {
@@ -577,6 +576,9 @@ extern "C" int favae_embed_bwd(const void* ids, int ids_are_64bit, const void* d
     FAVAE_REQUIRE(ids && dout && dweight && ws);
     if (!ok_sizes(T, V, C, dtype) || ((uintptr_t)ws & 15) || ((uintptr_t)dweight & 15)) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);
     const Plan p = plan(T, V, C);
+    const bool vec = vec_ok(dtype, C, 0, dout, dweight);
+    const int per = vec ? (dtype == F32 ? 256 : 512) : 64;                 // columns of a wave in the sums
+    if ((p.chunks * ((C + per - 1) / per) + 3) / 4 >= 1 << 24) return favae_prof_fail_(FAVAE_ERR_UNSUPPORTED);      // 2^32 threads a launch
     if (ws_bytes < p.total) return favae_prof_fail_(FAVAE_ERR_WORKSPACE);
     const hipStream_t s = (hipStream_t)stream;
     uint2* const buf[2] = {(uint2*)ws, (uint2*)((char*)ws + p.pairs)};
@@ -613,7 +615,6 @@ extern "C" int favae_embed_bwd(const void* ids, int ids_are_64bit, const void* d
             sorted = out;
         }
     }
-    const bool vec = vec_ok(dtype, C, 0, dout, dweight);
 #define GO(TY)                                                                                      \
     return vec ? go_sums<TY, true>(sorted, valid, dout, dweight, part, T, C, p, scale, s)              \
                : go_sums<TY, false>(sorted, valid, dout, dweight, part, T, C, p, scale, s)

@@ -145,3 +145,10 @@ def test_scales_that_leave_32_bits_in_powers_of_two_are_refused():
         assert (lib.favae_xattn_bwd_workspace(byref(d)) > 0) == ok
         if not ok:
             assert lib.favae_xattn_fwd(byref(d), 1 << 12, 1 << 12, 1 << 12, None, 1 << 12, None, None, None, 0, None) == 3
+
+
+def test_embedding_gradients_too_wide_for_a_launch_are_refused_before_the_first():
+    """the sums' launch is what they are too wide for; the sort before it must not have run"""
+    lib, P = favae_hip.load(), 1 << 12
+    for T, C, dt in ((4096, (1 << 24) - 1, 0), (1 << 17, 1 << 24, 1), (1 << 17, (1 << 22) + 1, 2)):
+        assert lib.favae_embed_bwd(P, 1, P, T, 4, C, dt, 1.0, -1, P, P, 1 << 62, None) == 3
