@@ -245,3 +245,60 @@ def test_block_over_no_states_is_the_identity_and_its_bias():
             assert bool(torch.isfinite(t).all()) and (n in ("y", "x", "proj.bias") or not t.any()), n
     for n, a, b in zip(names, results[0], results[2]):
         assert n == "states" or torch.equal(a, b), n
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("kind", ["tail", "holes", "empty"])
+@pytest.mark.parametrize("D", [40, 64, 128])
+def test_many_row_tiles_and_heads_over_many_keys(dtype, kind, D):
+    """the general form (more keys than stay in LDS) with ragged lengths, several row tiles of every head and many heads"""
+    dt = DT[dtype]
+    B, Lq, Lk, H, Hkv = 4, 333, 450, 8, 4
+    q, k, v, do = rnd((B, Lq, H, D), 1, dt), rnd((B, Lk, Hkv, D), 2, dt), rnd((B, Lk, Hkv, D), 3, dt), rnd((B, Lq, H, D), 4, dt)
+    pad = mask_of(kind, B, Lk, 6)
+    check(run(q, k, v, pad, D ** -0.5, do), *oracle(q, k, v, pad, D ** -0.5, do), dt)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_resident_keys_under_many_row_tiles(dtype):
+    """keys that stay in LDS while every workgroup goes through several row tiles, the last one partial; ragged lengths"""
+    dt = DT[dtype]
+    B, Lq, Lk, H, Hkv, D = 16, 1030, 70, 16, 16, 24
+    q, k, v, do = rnd((B, Lq, H, D), 1, dt), rnd((B, Lk, Hkv, D), 2, dt), rnd((B, Lk, Hkv, D), 3, dt), rnd((B, Lq, H, D), 4, dt)
+    pad = mask_of("empty", B, Lk, 6)
+    check(run(q, k, v, pad, 0.3, do), *oracle(q, k, v, pad, 0.3, do), dt)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("shape", [(1, 8, 70000, 1, 1, 64), (1, 70000, 64, 1, 1, 64), (1, 3, 30000, 2, 1, 128), (1, 20000, 3, 2, 1, 128), (2, 1, 40000, 4, 2, 32)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_hundreds_of_splits(shape, dtype):
+    """few queries over long keys (dq is summed over many splits) and few keys under many rows (dk and dv are)"""
+    dt = DT[dtype]
+    B, Lq, Lk, H, Hkv, D = shape
+    q, k, v, do = rnd((B, Lq, H, D), 1, dt), rnd((B, Lk, Hkv, D), 2, dt), rnd((B, Lk, Hkv, D), 3, dt), rnd((B, Lq, H, D), 4, dt)
+    pad = mask_of("holes", B, Lk, 5)
+    first = run(q, k, v, pad, D ** -0.5, do)
+    check(first, *oracle(q, k, v, pad, D ** -0.5, do), dt)
+    for n, t in run(q, k, v, pad, D ** -0.5, do).items():
+        assert torch.equal(t, first[n]), n
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("form", list(FORMS))
+def test_infinite_values_beside_padding(form, dtype):
+    """the pass with care sees the same mask: infinities and NaN among padded keys and one infinity among live ones, another sequence all
+    padding"""
+    K = ops()
+    Lq, Lk, G, D = FORMS[form]
+    q, k, v, _ = (t.to(DEV) for t in case(dtype, form))
+    pad = mask_of("holes", 2, Lk, 7).to(DEV)
+    pad[0], pad[1, 4] = True, False
+    k[pad], v[pad] = 0.0, 0.0
+    ref = K.cross_attention(q, k, v, pad)
+    k[pad], v[pad] = math.nan, -math.inf
+    v[1, 4, 1, 9] = math.inf
+    out = K.cross_attention(q, k, v, pad)
+    assert bool((out[1, :, G:, 9] == math.inf).all())
+    out[1, :, G:, 9] = ref[1, :, G:, 9]
+    assert torch.equal(out, ref)
