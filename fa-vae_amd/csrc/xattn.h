@@ -1528,17 +1528,27 @@ __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
     if (a.o32) put4<F32>(a.o32, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W * (1.f / SPARE));
 }
-// backward: out[i] = sum_s part[s][i], s ascending; n a multiple of 4.  8 splits of 0.5 M values: 5 us, about half of it the launch.
+// backward: out[i] = sum_s part[s][i], s ascending; n a multiple of 4.  8 splits of 0.5 M values: 5 us, about half of it the launch.  Sixteen
+// loads in flight: a small output has few threads, and one load at a time cost a memory latency a split (683 splits of 512 values: 172 us).
+template <int COUNT>
+__device__ __forceinline__ void add_splits(fx4& x, const float* part, int64_t n) {
+    fx4 y[COUNT];
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) y[i] = *reinterpret_cast<const fx4*>(part + i * n);
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += y[i][j];
+}
 template <int TY>
 __global__ __launch_bounds__(256) void join_sum_kernel(const float* part, void* out, int64_t n, int nsplit) {
     const int64_t e = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
     if (e >= n) return;
     fx4 x = *reinterpret_cast<const fx4*>(part + e);
-    for (int s = 1; s < nsplit; ++s) {
-        const fx4 y = *reinterpret_cast<const fx4*>(part + s * n + e);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] += y[j];
-    }
+    int s = 1;
+    for (; s + 16 <= nsplit; s += 16) add_splits<16>(x, part + s * n + e, n);
+    for (; s + 4 <= nsplit; s += 4) add_splits<4>(x, part + s * n + e, n);
+    for (; s < nsplit; ++s) add_splits<1>(x, part + s * n + e, n);
     put4<TY>(out, e, x[0], x[1], x[2], x[3]);
 }
 

@@ -12,16 +12,18 @@ struct Plan {
 
 // Splits the streamed axis of n elements into spans (multiples of 64, none under 128): the number of splits with the smallest estimate.
 // `base` workgroups exist without splits, `fit` of them run together on a CU, `tau` us is what one alone takes for 64 elements (and about
-// as much to start); two together take 1.5 times as long, three 1.7 times; a join takes 4 us and reads `bytes` a split at 7 TB/s.
+// as much to start); two together take 1.5 times as long, three 1.7 times; a join takes 4 us, reads `bytes` a split at 7 TB/s and waits
+// `wait` us a split: 0.042 in the sums of the backward pass (dq of 512 values: 31 us for 683 splits, 9 for 157; dk and dv make two),
+// 0.02 in the forward one (14 us for 512 splits of 8 rows).
 // Measured (us): fp32, 192 workgroups of 1500 keys x 64 columns: 104 in one span, 79 + 6 in 2, 83 + 6 in 3, 71 + 7 in 4, 75 + 10 in 8;
 // fp32, 40 of 5036 x 128: 801, 410 + 5, 283 + 5, 227 + 5, 124 + 5 in 8, 102 + 10 in 12; fp16, 288 of 515 x 80: 29, 28 + 8 in 2.
-void split_axis(int64_t base, int64_t n, int fit, double tau, double bytes, Plan& p) {
+void split_axis(int64_t base, int64_t n, int fit, double tau, double bytes, double wait, Plan& p) {
     static const double together[4] = {0.0, 1.0, 1.5, 1.7};
     const int64_t most = n / 128 < 1 ? 1 : n / 128 < MOST_SPLITS ? n / 128 : MOST_SPLITS, slots = 256 * (int64_t)fit;
     double best = 0.0;
     for (int64_t s = 1; s <= most && (s == 1 || base * s <= 4 * slots); s += 1 + s / 16) {
         const int64_t span = up((n + s - 1) / s, 64), ns = (n + span - 1) / span, full = base * ns / slots, rest = base * ns % slots;
-        const double t = (span / 64 + 1) * tau * (full * together[fit] + together[(rest + 255) / 256]) + (ns > 1 ? 4.0 + ns * bytes / 7e6 : 0.0);
+        const double t = (span / 64 + 1) * tau * (full * together[fit] + together[(rest + 255) / 256]) + (ns > 1 ? 4.0 + ns * (bytes / 7e6 + wait) : 0.0);
         if (s > 1 && t >= best) continue;
         best = t;
         p.span = (int)span;
@@ -55,7 +57,7 @@ Plan plan_fwd(const favae_xattn_desc* d) {
         p.tiles = (int)((tiles + span - 1) / span);
     } else {
         p.tiles = (int)((R + 127) / 128);
-        split_axis(p.tiles * heads, d->Lk, !f32 && d->D <= 64 ? 3 : 2, (f32 ? 2.2 : 0.6) * dim_pad(d->D) / 32, 4.0 * R * heads * d->D, p);
+        split_axis(p.tiles * heads, d->Lk, !f32 && d->D <= 64 ? 3 : 2, (f32 ? 2.2 : 0.6) * dim_pad(d->D) / 32, 4.0 * R * heads * d->D, 0.02, p);
     }
     return p;
 }
@@ -64,7 +66,8 @@ Plan plan_dq(const favae_xattn_desc* d) {
     Plan p{};
     p.tiles = (int)((R + 127) / 128);
     const bool f32 = d->dtype == F32;
-    split_axis(p.tiles * heads, d->Lk, f32 ? (d->D > 64 ? 1 : 2) : d->D <= 64 ? 3 : 2, (f32 ? 2.4 : 0.75) * dim_pad(d->D) / 32, 4.0 * R * heads * d->D, p);
+    split_axis(p.tiles * heads, d->Lk, f32 ? (d->D > 64 ? 1 : 2) : d->D <= 64 ? 3 : 2, (f32 ? 2.4 : 0.75) * dim_pad(d->D) / 32, 4.0 * R * heads * d->D,
+               0.042, p);
     return p;
 }
 Plan plan_dkv(const favae_xattn_desc* d) {
@@ -72,7 +75,7 @@ Plan plan_dkv(const favae_xattn_desc* d) {
     Plan p{};
     p.tiles = (d->Lk + 127) / 128;
     const bool f32 = d->dtype == F32;
-    split_axis(p.tiles * heads, R, f32 && d->D > 64 ? 1 : 2, (f32 ? 3.9 : 1.1) * dim_pad(d->D) / 32, 8.0 * heads * d->Lk * d->D, p);
+    split_axis(p.tiles * heads, R, f32 && d->D > 64 ? 1 : 2, (f32 ? 3.9 : 1.1) * dim_pad(d->D) / 32, 8.0 * heads * d->Lk * d->D, 0.084, p);
     return p;
 }
 
