@@ -79,12 +79,12 @@ __device__ __forceinline__ fx2 unpack2(unsigned u) {
 // x = hi + mid + lo, each rounded to nearest bf16; values beyond bf16's largest have that one as hi, and the planes still add up to them.
 // An infinity stands in the last plane alone: mma() multiplies that plane by the other operand's first one only, which has its value's sign
 // and is 0 where the value is, so the product is the infinity (or the NaN) of the definition.  In the first plane it would also meet the
-// other's lower planes, whose signs say nothing.  PROB: probabilities, which are neither.
-template <bool PROB = false>
+// other's lower planes, whose signs say nothing.  PLAIN: values that are neither (probabilities; tiles that were looked through).
+constexpr float MOST = 0x1.fep127f;
+template <bool PLAIN = false>
 __device__ __forceinline__ void split2(float a, float b, unsigned& hi, unsigned& mid, unsigned& lo) {
-    constexpr float MOST = 0x1.fep127f;
-    const bool ia = !PROB && __builtin_isinf(a), ib = !PROB && __builtin_isinf(b);
-    hi = PROB ? pack2<BF16>(a, b)
+    const bool ia = !PLAIN && __builtin_isinf(a), ib = !PLAIN && __builtin_isinf(b);
+    hi = PLAIN ? pack2<BF16>(a, b)
               : pack2<BF16>(__builtin_amdgcn_fmed3f(ia ? 0.f : a, -MOST, MOST), __builtin_amdgcn_fmed3f(ib ? 0.f : b, -MOST, MOST));
     const fx2 h = unpack2<BF16>(hi);
     const float ra = ia ? 0.f : a - h.x, rb = ib ? 0.f : b - h.y;          // a NaN gets here, whatever the median made of it
@@ -93,7 +93,7 @@ __device__ __forceinline__ void split2(float a, float b, unsigned& hi, unsigned&
     lo = pack2<BF16>(ia ? a : ra - m.x, ib ? b : rb - m.y);
 }
 // eight floats -> the planes of a fragment
-template <int TY, bool PROB = false>
+template <int TY, bool PLAIN = false>
 __device__ __forceinline__ Frag<Ty<TY>::PL> make_frag(const float* f) {
     Frag<Ty<TY>::PL> r;
     if constexpr (TY == F32) {
@@ -101,7 +101,7 @@ __device__ __forceinline__ Frag<Ty<TY>::PL> make_frag(const float* f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             unsigned a, b, c;
-            split2<PROB>(f[2 * i], f[2 * i + 1], a, b, c);
+            split2<PLAIN>(f[2 * i], f[2 * i + 1], a, b, c);
             h[i] = a; m[i] = b; l[i] = c;
         }
         r.p[0] = __builtin_bit_cast(s16x8, h);
@@ -258,6 +258,21 @@ template <int TY, int DP, int ROWS, int NT> struct Stage {
         return any;
     }
     __device__ __forceinline__ void store(short* t, int tid) const {
+        if constexpr (TY == F32) {                                         // one comparison for all of a wave's values, three instructions less for each
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const fx4 f = __builtin_bit_cast(fx4, r[i]);
+                most = fmaxf(fmaxf(fmaxf(most, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+            }
+            if (__builtin_amdgcn_ballot_w64(most > MOST)) put<false>(t, tid);
+            else put<true>(t, tid);
+        } else {
+            put<true>(t, tid);
+        }
+    }
+    template <bool PLAIN>
+    __device__ __forceinline__ void put(short* t, int tid) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int row = row_of(tid, i), col = col_of(tid, i);
@@ -268,8 +283,8 @@ template <int TY, int DP, int ROWS, int NT> struct Stage {
             if constexpr (TY == F32) {
                 unsigned h0, m0, l0, h1, m1, l1;
                 const fx4 f = __builtin_bit_cast(fx4, r[i]);
-                split2(f.x, f.y, h0, m0, l0);
-                split2(f.z, f.w, h1, m1, l1);
+                split2<PLAIN>(f.x, f.y, h0, m0, l0);
+                split2<PLAIN>(f.z, f.w, h1, m1, l1);
                 constexpr int PS = ROWS * DP;
                 *reinterpret_cast<uint2*>(p) = make_uint2(h0, h1);
                 *reinterpret_cast<uint2*>(p + PS) = make_uint2(m0, m1);
