@@ -141,6 +141,14 @@ __device__ __forceinline__ f32x16 mma(const Frag<Ty<TY>::PL>& a, const Frag<Ty<T
 // depends on one would be looped over
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// 0, which the compiler does not know: a second pass whose bounds contain it shares no addresses with the first, and its registers hold none
+// for it (token to long states 94.5 -> 92.5 us)
+__device__ __forceinline__ int hidden_zero() {
+    int z = 0;
+    asm volatile("" : "+s"(z));
+    return z;
+}
+
 __device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
@@ -456,6 +464,16 @@ template <int BK> struct KeyBits {
 // All leave the bits of everything that was a number.
 template <int TY> constexpr float SMALL = TY == F16 ? 1.f : 0x1p-40f;
 template <int TY, bool CARE> __device__ __forceinline__ float prob(float x) { return CARE ? exp2_f(x) * SMALL<TY> : exp2_f(x); }
+// whether any of the first NW waves says so, to all threads; `flags`: NW ints of LDS.  One barrier: every wave is done with the tiles, too.
+template <int NW> __device__ __forceinline__ bool some_wave(bool mine, int w, int lane, int* flags) {
+    const bool any = __builtin_amdgcn_ballot_w64(mine) != 0;
+    if (w < NW && lane == 0) flags[w] = any;
+    __syncthreads();
+    int r = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) r |= flags[i];
+    return uniform(r) != 0;
+}
 // the exponent of a row's probabilities is c (s - r) + sh
 struct Ref {
     float r, sh;
@@ -518,7 +536,7 @@ template <int TY, int DP, bool KEYW> struct FwdCfg {
     static constexpr int BUFS = bufs_of(TILE, WAVES, PRE);
     static constexpr int RED = KEYW ? NW * DP * 32 * 2 : 0;               // joined results (fp32, in 16-bit units), over the tiles
     static constexpr int LEN = 2 * TILE * BUFS > RED ? 2 * TILE * BUFS : RED;
-    static constexpr size_t LDS = LEN * 2 + BUFS * BK * 4 + 64 * 4 * NW + 16;
+    static constexpr size_t LDS = LEN * 2 + BUFS * BK * 4 + 64 * 4 * NW + 4 * 4;
 };
 
 template <int TY, int DP, bool KEYW>
@@ -655,20 +673,25 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
         }
     };
     pass(std::false_type{});
-    float lt = l + other_half(l);
-    if (uniform(__syncthreads_or(not_finite(o) || (lt == 0.f && m > -INFINITY)))) {
-        if (C::PRE) fetch(k0);
-        pass(std::true_type{});
-        up = 1.f / SMALL<TY>;
+    float lt;
+    const auto odd = [&] {                                                  // KEYW: the waves are joined, row statistics first
         lt = l + other_half(l);
-    }
-    if constexpr (KEYW) {
-        // join the waves: row statistics first, then each wave's scaled accumulators through LDS
-        if (half == 0 && w < C::NW) {
+        if (KEYW && half == 0 && w < C::NW) {
             stat[w * 32 + lane] = m;
             stat[(C::NW + w) * 32 + lane] = lt;
         }
-        __syncthreads();                                                    // also: every wave is done with the tiles
+        return some_wave<C::NW>(not_finite(o) || (lt == 0.f && m > -INFINITY), w, lane, red);
+    };
+    if (__builtin_expect(odd(), 0)) {
+        const int z = hidden_zero();
+        kend += z;
+        if (C::PRE) fetch(k0 + z);
+        pass(std::true_type{});
+        up = 1.f / SMALL<TY>;
+        odd();
+    }
+    if constexpr (KEYW) {
+        // each wave's scaled accumulators through LDS
         float M = -INFINITY, L = 0.f;
 #pragma unroll
         for (int i = 0; i < C::NW; ++i) M = fmaxf(M, stat[i * 32 + (lane & 31)]);
@@ -1085,18 +1108,22 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
         x += __shfl_xor(x, 16, 64);
         return x + __shfl_xor(x, 32, 64);
     };
-    float lt = total(l);
-    if (uniform(__syncthreads_or(not_finite(o) || (lt == 0.f && m > -INFINITY)))) {
-        fetch(k0);
+    const auto odd = [&] {
+        const float lt = total(l);
+        if (quad == 0 && w < C::NW) {
+            stat[w * 16 + row] = m;
+            stat[(C::NW + w) * 16 + row] = lt;
+        }
+        return some_wave<C::NW>(not_finite(o) || (lt == 0.f && m > -INFINITY), w, lane, red);
+    };
+    if (__builtin_expect(odd(), 0)) {
+        const int z = hidden_zero();
+        kend += z;
+        fetch(k0 + z);
         pass(std::true_type{});
         up = 1.f / SMALL<TY>;
-        lt = total(l);
+        odd();
     }
-    if (quad == 0 && w < C::NW) {
-        stat[w * 16 + row] = m;
-        stat[(C::NW + w) * 16 + row] = lt;
-    }
-    __syncthreads();                                                        // also: every wave is done with the tiles
     float M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int i = 0; i < C::NW; ++i) M = fmaxf(M, stat[i * 16 + row]);
