@@ -464,6 +464,11 @@ template <int BK> struct KeyBits {
 // All leave the bits of everything that was a number.
 template <int TY> constexpr float SMALL = TY == F16 ? 1.f : 0x1p-40f;
 template <int TY, bool CARE> __device__ __forceinline__ float prob(float x) { return CARE ? exp2_f(x) * SMALL<TY> : exp2_f(x); }
+// A row whose probabilities sum to 0 has no keys, and gives zeros, or keys whose scores are all -infinity, and gives the NaN of the formula
+// (an infinite query makes one of every score that is not).  A split writes zeros for both, and NO_SCORE as the second one's log-sum.
+constexpr float NO_SCORE = -3.402823466e38f;
+__device__ __forceinline__ float no_sum(bool keys) { return keys ? __builtin_nanf("") : 0.f; }
+__device__ __forceinline__ float no_lse(bool keys) { return keys ? __builtin_nanf("") : INFINITY; }
 // whether any of the first NW waves says so, to all threads; `flags`: NW ints of LDS.  One barrier: every wave is done with the tiles, too.
 template <int NW> __device__ __forceinline__ bool some_wave(bool mine, int w, int lane, int* flags) {
     const bool any = __builtin_amdgcn_ballot_w64(mine) != 0;
@@ -702,7 +707,7 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
             L += x == -INFINITY ? 0.f : exp2_f((x - mr) * a.c) * stat[(C::NW + i) * 32 + (lane & 31)];
         }
         const float f = m == -INFINITY ? 0.f : exp2_f((m - mr) * a.c);
-        const float inv = L == 0.f ? 0.f : f / L;
+        const float inv = L == 0.f ? no_sum(kend > k0 && a.nsplit == 1) : f / L;
         float* acc = reinterpret_cast<float*>(lds);
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t)
@@ -711,9 +716,9 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
                 if (w < C::NW) acc[(w * DP + 32 * t + 8 * (i >> 2) + 4 * half + (i & 3)) * 32 + (lane & 31)] = o[t][i] * inv;
         __syncthreads();
         if (w == 0 && half == 0 && row < a.R) {
-            const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L * up) - T::FSHIFT);
+            const float ls = L == 0.f ? (kend > k0 ? NO_SCORE : -INFINITY) : M * a.c + (__builtin_amdgcn_logf(L * up) - T::FSHIFT);
             if (a.nsplit > 1) a.part_lse[((int64_t)split * a.B * a.Hkv + bh) * a.R + row] = ls;
-            else if (a.lse) a.lse[(int64_t)bh * a.R + row] = L == 0.f ? INFINITY : ls;
+            else if (a.lse) a.lse[(int64_t)bh * a.R + row] = L == 0.f ? no_lse(kend > k0) : ls;
         }
         const int nq = a.D / 4;
         for (int e = tid; e < 32 * nq; e += C::NT) {
@@ -733,14 +738,14 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
             }
         }
     } else {
-        const float inv = lt == 0.f ? 0.f : 1.f / lt;
-        const float ls = lt == 0.f ? -INFINITY : m * a.c + (__builtin_amdgcn_logf(lt * up) - T::FSHIFT);
+        const float inv = lt == 0.f ? no_sum(kend > k0 && a.nsplit == 1) : 1.f / lt;
+        const float ls = lt == 0.f ? (kend > k0 ? NO_SCORE : -INFINITY) : m * a.c + (__builtin_amdgcn_logf(lt * up) - T::FSHIFT);
         const int64_t flat = ((int64_t)split * a.B * a.Hkv + bh) * a.R + row;
         const bool in = row < a.R;
         const OutRows to_row(a, bh, row0);
         if (half == 0 && in) {
             if (a.nsplit > 1) a.part_lse[flat] = ls;
-            else if (a.lse) a.lse[(int64_t)bh * a.R + row] = lt == 0.f ? INFINITY : ls;
+            else if (a.lse) a.lse[(int64_t)bh * a.R + row] = lt == 0.f ? no_lse(kend > k0) : ls;
         }
         // 32-bit results: a lane's four consecutive columns are one 16-byte store
         if (TY == F32 || a.nsplit > 1 || a.o32) {
@@ -878,9 +883,9 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
                 }
             }
         l += other_half(l);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? no_sum(keys) : 1.f / l;
         const OutRows to_row(a, bh, rt);
-        if (half == 0 && in && a.lse) a.lse[(int64_t)bh * a.R + row] = l == 0.f ? INFINITY : m * a.c + (__builtin_amdgcn_logf(l) - shift);
+        if (half == 0 && in && a.lse) a.lse[(int64_t)bh * a.R + row] = l == 0.f ? no_lse(keys) : m * a.c + (__builtin_amdgcn_logf(l) - shift);
         if (TY == F32 || a.o32) {
             float* const to = TY == F32 ? (float*)a.o : a.o32;
             const int64_t at = in ? to_row.at(a, bh, lane & 31) : 0;
@@ -1134,7 +1139,7 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
         L += x == -INFINITY ? 0.f : exp2_f((x - mr) * a.c) * stat[(C::NW + i) * 16 + row];
     }
     const float f = m == -INFINITY ? 0.f : exp2_f((m - mr) * a.c);
-    const float inv = L == 0.f ? 0.f : f / L;
+    const float inv = L == 0.f ? no_sum(kend > k0 && a.nsplit == 1) : f / L;
     float* acc = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t)
@@ -1143,9 +1148,9 @@ __global__ __launch_bounds__(256, 2) void fwd_token_kernel(const Args a) {
             if (w < C::NW) acc[(w * DP + 16 * t + 4 * quad + i) * 16 + row] = o[t][i] * inv;
     __syncthreads();
     if (w == 0 && quad == 0 && row < a.R) {
-        const float ls = L == 0.f ? -INFINITY : M * a.c + (__builtin_amdgcn_logf(L * up) - T::FSHIFT);
+        const float ls = L == 0.f ? (kend > k0 ? NO_SCORE : -INFINITY) : M * a.c + (__builtin_amdgcn_logf(L * up) - T::FSHIFT);
         if (a.nsplit > 1) a.part_lse[((int64_t)split * heads + bh) * a.R + row] = ls;
-        else if (a.lse) a.lse[(int64_t)bh * a.R + row] = L == 0.f ? INFINITY : ls;
+        else if (a.lse) a.lse[(int64_t)bh * a.R + row] = L == 0.f ? no_lse(kend > k0) : ls;
     }
     const int nq = a.D / 4;
     for (int e = tid; e < a.R * nq; e += C::NT) {
@@ -1519,11 +1524,11 @@ __global__ __launch_bounds__(256) void join_few_kernel(const Args a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = fmaf(wgt, y[s][j], x[j]);
     }
-    const float inv = W == 0.f ? 0.f : 1.f / W;
+    const float inv = W == 0.f ? 0.f : M == NO_SCORE ? no_sum(true) : 1.f / W;
     const int64_t at = out_at(a, (int)(fr / a.R), (int)(fr % a.R)) + d;
     put4<TY>(a.o, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     if (a.o32) put4<F32>(a.o32, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W * (1.f / SPARE));
+    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M == NO_SCORE ? no_lse(true) : M + __builtin_amdgcn_logf(W * (1.f / SPARE));
 }
 
 // Many splits: a workgroup owns a row, its threads take four columns of every (256 / columns)-th split, so that one latency covers many
@@ -1546,7 +1551,7 @@ __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
     if (lane == 0) red[4 + w] = W;
     __syncthreads();
     W = red[4] + red[5] + red[6] + red[7];
-    const float inv = W == 0.f ? 0.f : 1.f / W;
+    const float inv = W == 0.f ? 0.f : M == NO_SCORE ? no_sum(true) : 1.f / W;
     const int nq = a.D / 4, ng = 256 / nq, g = tid / nq, d = 4 * (tid % nq);
     fx4 x = {0.f, 0.f, 0.f, 0.f};
     if (g < ng)
@@ -1568,7 +1573,7 @@ __global__ __launch_bounds__(256) void join_fwd_kernel(const Args a) {
     const int64_t at = out_at(a, bh, r) + d;
     put4<TY>(a.o, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     if (a.o32) put4<F32>(a.o32, at, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M + __builtin_amdgcn_logf(W * (1.f / SPARE));
+    if (d == 0 && a.lse) a.lse[fr] = W == 0.f ? INFINITY : M == NO_SCORE ? no_lse(true) : M + __builtin_amdgcn_logf(W * (1.f / SPARE));
 }
 // backward: out[i] = sum_s part[s][i], s ascending; n a multiple of 4.  8 splits of 0.5 M values: 5 us, about half of it the launch.  Sixteen
 // loads in flight: a small output has few threads, and one load at a time cost a memory latency a split (683 splits of 512 values: 172 us).

@@ -302,3 +302,35 @@ def test_infinite_values_beside_padding(form, dtype):
     assert bool((out[1, :, G:, 9] == math.inf).all())
     out[1, :, G:, 9] = ref[1, :, G:, 9]
     assert torch.equal(out, ref)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("form", list(FORMS))
+def test_rows_without_a_score_and_nan_inputs(form, dtype):
+    """a row that has keys, all of whose scores are -infinity, is the formula's NaN (0 / 0), whatever stands beside the last key; a NaN in a
+    query is its row's, in a key its head's, in a value its column's"""
+    K = ops()
+    Lq, Lk, G, D = FORMS[form]
+    q, k, v, _ = (t.to(DEV) for t in case(dtype, form))
+    k[..., 5] = k[..., 5].abs() + 0.125
+    ref = K.cross_attention(q, k, v)
+    q2, k2, v2 = q.clone(), k.clone(), v.clone()
+    q2[1, Lq // 2, 0, 5], q2[0, 0, -1, 3] = -math.inf, math.nan
+    out = K.cross_attention(q2, k, v)
+    assert bool(out[1, Lq // 2, 0].isnan().all()) and bool(out[0, 0, -1].isnan().all())
+    out[1, Lq // 2, 0], out[0, 0, -1] = ref[1, Lq // 2, 0], ref[0, 0, -1]
+    assert torch.equal(out, ref)
+    some = k.clone()                                                             # the same by infinite keys; one key without an infinity is enough
+    some[:, :, 0, 5] = -math.inf
+    q3 = q.clone()
+    q3[..., 5] = q3[..., 5].abs() + 0.125
+    assert bool(K.cross_attention(q3, some, v)[:, :, :G].isnan().all())
+    some[1, 40, 0] = k[1, 40, 0]
+    # p v / p, p near 1: the product, the reciprocal, its product and a join's are off by 2^-24 each; p and the result are rounded to 16 bits
+    lim = (4 * 2.0 ** -24 + (0 if dtype == "fp32" else 2 * half_step(DT[dtype]))) * v[1, 40, 0].double().abs()
+    assert bool(((K.cross_attention(q3, some, v)[1, :, :G].double() - v[1, 40, 0].double()).abs() <= lim).all())
+    k2[0, Lk // 2, 1, 7], v2[0, 3, 0, 2] = math.nan, math.nan
+    out = K.cross_attention(q, k2, v2)
+    assert bool(out[0, :, G:].isnan().all()) and bool(out[0, :, :G, 2].isnan().all())
+    out[0, :, G:], out[0, :, :G, 2] = ref[0, :, G:], ref[0, :, :G, 2]
+    assert torch.equal(out, ref)
