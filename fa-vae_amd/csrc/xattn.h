@@ -13,7 +13,8 @@
 //     dropped ones are below 2^-24 of the operands' product: 2.7 x the rate of the fp32 matrix instruction.
 //   * 16-bit elements: probabilities, and score gradients backward, are rounded to the element type for the second product: one MFMA
 //     instead of the two that a second plane would take, for half a step of the type per probability (results are then off by about 1.4
-//     times what the rounding of the result alone costs).  Sums, maxima, log-sums and accumulators are fp32.
+//     times what the rounding of the result alone costs).  The forward forms of up to 64 rows are bound by the keys' bytes and have the time
+//     for that second plane, so a row among few is rounded once only.  Sums, maxima, log-sums and accumulators are fp32.
 // Rows that share a key / value head are packed: row r = g * Lq + i is query i of the g-th head of the group.
 // Times at the kernels below are the kernel's alone, between the slowest and the fastest card measured; rates count 4, 6 and 8 D
 // operations a score for the forward pass, dq, and dk and dv.
@@ -527,7 +528,8 @@ __device__ __forceinline__ f32x16 scores(const short* t, int row0, const Frag<Ty
 // six products: 16 heads x 2048 x 2048 x 128 in two spans 181-196 us, 175-190 TFLOP/s, six times that on the matrix pipe; 10 us to join.
 // One 32-row group a wave, 3 waves a SIMD with 16-bit elements of up to 64 columns (V's first half is read ahead of the exponentials: 3 %).
 // 64 rows a wave took the same time, two groups with interleaved exponentials 10 % more, four waves (32 keys at a time) 6 %, the next
-// tile's stores between the products 15 %, sums by products with ones 4 %.
+// tile's stores between the products 15 %, sums by products with ones 4 %.  fp32 of 128 columns spills 23 registers (72 bytes of scratch a
+// lane, of which the key loop reads some again); the other forms spill none.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP, bool KEYW> struct FwdCfg {
     static constexpr int NT = 256;
@@ -788,8 +790,8 @@ __global__ __launch_bounds__((FwdCfg<TY, DP, KEYW>::NT), (FwdCfg<TY, DP, KEYW>::
 // -------------------------------------------------------------------------------------------------------------------------------------
 // Forward over few keys (a prompt): all of them stay in LDS and a workgroup goes through many row tiles, each wave by itself without a
 // barrier, the next tile's queries on their way.  One maximum per row, nothing is rescaled.  What is left is reading q and writing o.
-// bf16, 128 heads x 4096 rows x 77 keys x 64 columns: 33 us, 4.1 TB/s of q and o (fwd_kernel: 46); fp32, 256 heads x 256 x 77 x 64: 19 us,
-// there each wave has one row tile and waits for the keys' planes.
+// bf16 and fp16, 128 heads x 4096 rows x 77 keys x 64 columns: 33 us, 4.1 TB/s of q and o (fwd_kernel: 46); fp32, 256 heads x 256 x 77 x 64:
+// 22 us, there each wave has one row tile and waits for the keys' planes.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP> struct ShortCfg {
     static constexpr int NT = 256, KEYS = TY == F32 ? 96 : 128, KT = KEYS / 32;
@@ -935,8 +937,9 @@ __global__ __launch_bounds__(256, 2) void fwd_short_kernel(const Args a) {
 // Forward of up to 16 rows a head group (a decoding step): bound by the bytes of K and V.  16x16x32 MFMAs hold the 16 rows in half the
 // registers of the 32-row form, so that two workgroups of 128 keys a tile share a CU and one's loads run under the other's arithmetic.
 // Each wave takes 32 keys of the tile: lane l holds row l % 16 and keys 4 (l / 16) + i and 16 + 4 (l / 16) + i, which are also the
-// contraction slots of the second product.  fp16, 4 x 8 heads of 4 rows x 30011 keys x 128 columns in 16 spans: 87 us, 5.7 TB/s (32-row
-// form: 125), and 5 us for the join; bf16, 256 heads of one row x 77 keys: 6 us, of which a launch and two memory latencies are 4.
+// contraction slots of the second product.  fp16, 4 x 8 heads of 4 rows x 30011 keys x 128 columns of ragged sequences (400 MB) in 16 spans:
+// 88 us, 4.6 TB/s (32-row form: 125), and 5 us for the join; fp32 242 us for 800 MB, 3.3 TB/s, where two of the four waves only load; bf16,
+// 256 heads of one row x 77 keys: 6 us, of which a launch and two memory latencies are 4.
 // The matrix pipe has time here: probabilities are rounded to two planes, products of both are summed.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY> __device__ __forceinline__ fx4 mma16_1(s16x8 a, s16x8 b, fx4 c) {
@@ -1338,7 +1341,9 @@ template <int TY, int DP> struct DkvCfg {
     static constexpr int WAVES = TY == F32 && DP > 64 ? 1 : 2;
     // more than 64 columns (fp32: 32): the values' rows stay in LDS, their operands are read again for every tile, and dp is formed after
     // the probabilities are used; a wave's registers hold no more beside both accumulators.  bf16, 64 heads x 1024 x 1024: 128 columns
-    // 148 -> 87 us (790 TFLOP/s, two waves a SIMD instead of one), 96 columns 87 -> 76 us; fp32 the same time within 2 %, without spills.
+    // 148 -> 87 us (790 TFLOP/s, two waves a SIMD instead of one), 96 columns 87 -> 76 us; fp32 the same time within 2 %.  At 128 columns
+    // 16-bit elements still spill 8 (bf16) and 12 (fp16) registers, 36 and 52 bytes of scratch that the row loop reads again, and fp32 9
+    // into the accumulation registers.
     static constexpr int VALS = TIGHT ? tile_len<TY, DP, KEYS>() : 0;
     static constexpr int TILE = tile_len<TY, DP, BR>();
     static constexpr int BUFS = TIGHT ? 1 : bufs_of(TILE, WAVES, true);

@@ -1995,6 +1995,9 @@ def cross_attention(q, k, v, key_padding_mask=None, scale=None):
     infinite value.
     Scores may be of any finite size.  The backward pass forms the probabilities again from 32-bit log-sums, half a step of which is a
     relative error of |score| / 2^24: scores of 10^4 and more cost gradients their precision, scores above 10^9 their meaning.
+    Sums and softmax statistics are fp32 and a result is rounded once.  16-bit types: probabilities, and score gradients backward, enter
+    their second product rounded to the type, too (forward with up to 64 rows of a key head: to twice its bits), which makes the error of
+    many rows about 1.4 times that of the result's rounding alone.
     Lq = 1 (a decoding step) and long keys run the same call: the keys are split over the chip.  Differentiable in q, k, v, once and
     backward: forward-mode tangents raise, as second derivatives do."""
     _require_float_gpu("cross_attention", q, k, v)

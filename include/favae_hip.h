@@ -519,6 +519,9 @@ int favae_gn_act_bwd_tiles(const float* da, const float* x, const float* gamma, 
  * length: that one is at least D and below 2^24 bytes); o, dout and the gradients are dense (H * D elements below 2^24 bytes too).
  * D % 8 == 0, 8 <= D <= 128, 0 < scale < 2.3e38.  key_padding_mask: NULL, or B rows of Lk bytes pad_sb bytes apart, nonzero = this key is padding:
  * what its rows of k and v hold (infinities, NaN) reaches no result and its gradients are zeros.
+ * Infinities and NaN that are not padding do what the formula makes of them; scores of any finite size give the forward pass's value.
+ * 16-bit elements: probabilities and score gradients enter their second product rounded to the type (forward passes of up to 64 rows of a
+ * key head: to twice its bits).
  * Every data pointer is 16-byte aligned.  Results do not depend on anything but the arguments (no atomics on floats). */
 typedef struct {
     int32_t B, Lq, Lk, H, Hkv, D, dtype;
@@ -526,7 +529,8 @@ typedef struct {
     int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, pad_sb;
 } favae_xattn_desc;
 /* Forward.  o32 (may be NULL): o before its rounding, fp32; lse (may be NULL): B * H * Lq floats.  The backward pass wants both (for
- * fp32 elements o32 may be o itself).  Workspace: 0 bytes unless few rows attend to many keys (the keys are then split). */
+ * fp32 elements o32 may be o itself).  The workspace depends on how the call is split over the chip, many rows as well as few: ask for its
+ * size with the same descriptor (0: none is needed). */
 size_t favae_xattn_fwd_workspace(const favae_xattn_desc* d);
 int favae_xattn_fwd(const favae_xattn_desc* d, const void* q, const void* k, const void* v, const uint8_t* key_padding_mask, void* o,
                     float* o32, float* lse, void* ws, size_t ws_bytes, favae_stream_t stream);
