@@ -528,8 +528,8 @@ __device__ __forceinline__ f32x16 scores(const short* t, int row0, const Frag<Ty
 // six products: 16 heads x 2048 x 2048 x 128 in two spans 181-196 us, 175-190 TFLOP/s, six times that on the matrix pipe; 10 us to join.
 // One 32-row group a wave, 3 waves a SIMD with 16-bit elements of up to 64 columns (V's first half is read ahead of the exponentials: 3 %).
 // 64 rows a wave took the same time, two groups with interleaved exponentials 10 % more, four waves (32 keys at a time) 6 %, the next
-// tile's stores between the products 15 %, sums by products with ones 4 %.  fp32 of 128 columns spills 23 registers (72 bytes of scratch a
-// lane, of which the key loop reads some again); the other forms spill none.
+// tile's stores between the products 15 %, sums by products with ones 4 %.  fp32 of 128 columns spills 24 registers (72 bytes of scratch a
+// lane; six loads of it a tile of 96 MFMAs); the other forms spill none.
 // -------------------------------------------------------------------------------------------------------------------------------------
 template <int TY, int DP, bool KEYW> struct FwdCfg {
     static constexpr int NT = 256;
