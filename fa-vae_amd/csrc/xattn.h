@@ -143,7 +143,7 @@ __device__ __forceinline__ f32x16 mma(const Frag<Ty<TY>::PL>& a, const Frag<Ty<T
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // 0, which the compiler does not know: a second pass whose bounds contain it shares no addresses with the first, and its registers hold none
-// for it (token to long states 94.5 -> 92.5 us)
+// for it (fwd_token_kernel and its join, fp16, 4 x 8 heads of 4 rows x 30011 keys x 128 columns: 94.5 -> 92.5 us)
 __device__ __forceinline__ int hidden_zero() {
     int z = 0;
     asm volatile("" : "+s"(z));
